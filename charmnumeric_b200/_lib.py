@@ -52,6 +52,8 @@ SIGNATURES = {
     "cn_get": (C.c_int, [_P, C.c_int, C.c_int, C.c_int, C.c_int64, C.c_int, _P]),
     "cn_get_local": (C.c_int, [_P, C.c_int, _I64P, _I64P, C.c_int64, _P]),
     "cn_put": (C.c_int, [_P, C.c_int, C.c_int, _I64P, C.c_int, _P]),
+    "cn_put_device": (C.c_int, [_P, C.c_int, C.c_int, _I64P, C.c_int, _P, _P]),
+    "cn_device_array": (C.c_int, [_P, C.c_int, C.POINTER(_P), C.POINTER(_P)]),
     "cn_get_root": (C.c_int, [_P, C.c_int, C.c_int, C.c_int, C.c_int64, C.c_int, C.c_int, _P]),
     "cn_put_local": (C.c_int, [_P, C.c_int, C.c_int, _I64P, C.c_int, C.c_int64, _P]),
     "cn_execute_node": (C.c_int, [_P, C.c_char_p, C.c_int64]),

@@ -18,8 +18,9 @@ BUILD = HERE / "_build"
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 HOST_SOURCES = ["wire.cpp", "lower.cpp", "fuse.cpp", "regions.cpp", "decomp.cpp", "codegen.cpp", "jit.cpp", "comm.cpp", "context.cpp",
-                "executor.cpp", "capi.cpp"]
-CUDA_SOURCES = ["kernels.cu", "noalloc.cu"]
+                "executor.cpp", "sequence.cpp", "capi.cpp"]
+SEQUENCE_SOURCES = ["rms_norm.cu", "causal_conv.cu", "selective_scan.cu", "sample.cu"]
+CUDA_SOURCES = ["kernels.cu", "noalloc.cu"] + SEQUENCE_SOURCES
 
 
 def _embed():
@@ -27,6 +28,8 @@ def _embed():
     dev = (CSRC / "cn_device.cuh").read_text()
     tab = (CSRC / "cn_exp_table.inc").read_text()
     aot = hashlib.sha256((CSRC / "kernels.cu").read_bytes() + (CSRC / "kernels.hpp").read_bytes()).hexdigest()[:8]
+    seq = hashlib.sha256(b"".join((CSRC / s).read_bytes() for s in SEQUENCE_SOURCES + ["sequence.cuh", "sequence.hpp"])).hexdigest()[:8]
+
     def lit(text):
         # split into chunks: one raw string literal must stay below compiler limits
         parts = [text[i:i + 8000] for i in range(0, len(text), 8000)]
@@ -36,7 +39,8 @@ def _embed():
             "const char* const kExpTableText =\n" + lit(tab) + ";\n"
             # the kernels built ahead of time (matvec, dot, halo copies) are identified in
             # profile labels by a digest of their source
-            'const char* const kAotSourceDigest = "' + aot + '";\n}\n')
+            'const char* const kAotSourceDigest = "' + aot + '";\n'
+            'const char* const kSequenceSourceDigest = "' + seq + '";\n}\n')
     path = BUILD / "embedded_headers.cpp"
     if not path.exists() or path.read_text() != body:
         path.write_text(body)

@@ -6,7 +6,8 @@ import numpy as np
 from . import _lib, wire
 
 NP_DTYPES = {wire.F32: np.dtype("float32"), wire.F64: np.dtype("float64"),
-             wire.I32: np.dtype("int32"), wire.I64: np.dtype("int64")}
+             wire.I32: np.dtype("int32"), wire.I64: np.dtype("int64"),
+             wire.F16: np.dtype("float16"), wire.I8: np.dtype("int8")}
 WIRE_DTYPES = {v: k for k, v in NP_DTYPES.items()}
 
 
@@ -161,6 +162,19 @@ class Context:
         shape = (C.c_int64 * host.ndim)(*host.shape)
         self._check(self._lib.cn_put(self._h, int(name), host.ndim, shape, WIRE_DTYPES[host.dtype],
                                      host.ctypes.data_as(C.c_void_p)))
+
+    def put_device(self, name, shape, dtype, pointer, stream=0):
+        """Copy a whole dense array from device memory that another library owns; ``stream`` is
+        the stream its values were made on."""
+        cshape = (C.c_int64 * len(shape))(*shape)
+        self._check(self._lib.cn_put_device(self._h, int(name), len(shape), cshape, WIRE_DTYPES[np.dtype(dtype)],
+                                            C.c_void_p(pointer), C.c_void_p(stream)))
+
+    def device_array(self, name):
+        """(address of this rank's rows of an array, stream of the context's work), as integers."""
+        data, stream = C.c_void_p(), C.c_void_p()
+        self._check(self._lib.cn_device_array(self._h, int(name), C.byref(data), C.byref(stream)))
+        return data.value, stream.value
 
     # ---- measurement ----
     def timer_start(self):

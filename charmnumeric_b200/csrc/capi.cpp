@@ -94,6 +94,17 @@ int cn_put(cn_context* ctx, int name, int ndims, const int64_t* shape, int dtype
     return ctx->impl.put(name, ndims, shape, dtype, host);
 }
 
+int cn_put_device(cn_context* ctx, int name, int ndims, const int64_t* shape, int dtype, const void* data,
+                  void* stream) {
+    if (!ctx || !shape) return cn::CN_ERR_INVALID_ARGUMENT;
+    return ctx->impl.put_device(name, ndims, shape, dtype, data, (cudaStream_t)stream);
+}
+
+int cn_device_array(cn_context* ctx, int name, void** data, void** stream) {
+    if (!ctx) return cn::CN_ERR_INVALID_ARGUMENT;
+    return ctx->impl.device_array(name, data, stream);
+}
+
 int cn_get_root(cn_context* ctx, int ndims, int epoch, int name, int64_t count, int dtype, int root,
                 void* out) {
     (void)ndims;

@@ -33,6 +33,13 @@ enum Opcode : int {
     OP_ABS = 12,
     OP_SUM = 13,    // sum of all elements of one array -> size-1 array
     OP_RANDU = 14,  // seeded uniform fill: operands (seed, lo, hi) as literal scalars
+    // operators of sequence models (sequence.cpp): one root with the operands (a literal scalar in
+    // the place of one that is left out), followed by a NOOP root for every further result
+    OP_RMS_NORM = 15,
+    OP_CAUSAL_CONV = 16,
+    OP_SELECTIVE_SCAN = 17,
+    OP_SAMPLE = 18,
+    OP_CONVERT = 19,  // element type conversion, and values of 8-bit codes with scales
 };
 
 inline bool is_binary_elementwise(int op) { return op >= OP_ADD && op <= OP_DIV; }
@@ -41,9 +48,14 @@ inline bool is_unary_elementwise(int op) {
 }
 inline bool is_elementwise(int op) { return is_binary_elementwise(op) || is_unary_elementwise(op); }
 
-enum DType : int { DT_F32 = 0, DT_F64 = 1, DT_I32 = 2, DT_I64 = 3 };
-inline int dtype_size(int dt) { return (dt == DT_F64 || dt == DT_I64) ? 8 : 4; }
-inline bool dtype_valid(int dt) { return dt >= 0 && dt <= 3; }
+// F16 and I8 are storage types: arrays of them can be created, filled, copied, converted and moved,
+// and the sequence operators read and write them; there is no arithmetic on them.
+enum DType : int { DT_F32 = 0, DT_F64 = 1, DT_I32 = 2, DT_I64 = 3, DT_F16 = 4, DT_I8 = 5 };
+inline int dtype_size(int dt) {
+    return (dt == DT_F64 || dt == DT_I64) ? 8 : dt == DT_F16 ? 2 : dt == DT_I8 ? 1 : 4;
+}
+inline bool dtype_valid(int dt) { return dt >= DT_F32 && dt <= DT_I64; }     // types with arithmetic
+inline bool dtype_storable(int dt) { return dt >= DT_F32 && dt <= DT_I8; }   // types an array may have
 
 // Status codes returned through the C ABI (the reference aborts the process instead).
 enum Status : int {

@@ -18,7 +18,7 @@ typedef void* ncclComm_t;
 struct ncclUniqueId_ {
     char internal[128];
 };
-enum { kNcclInt32 = 2, kNcclInt64 = 4, kNcclFloat32 = 7, kNcclFloat64 = 8, kNcclSum = 0 };
+enum { kNcclInt8 = 0, kNcclInt32 = 2, kNcclFloat16 = 6, kNcclInt64 = 4, kNcclFloat32 = 7, kNcclFloat64 = 8, kNcclSum = 0 };
 
 struct NcclApi {
     void* handle = nullptr;
@@ -73,6 +73,8 @@ int nccl_type(int dtype) {
         case DT_F32: return kNcclFloat32;
         case DT_F64: return kNcclFloat64;
         case DT_I32: return kNcclInt32;
+        case DT_F16: return kNcclFloat16;
+        case DT_I8: return kNcclInt8;
         default: return kNcclInt64;
     }
 }

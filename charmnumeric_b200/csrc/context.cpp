@@ -226,7 +226,7 @@ void Context::free_buffer(Buffer* b) {
 int Context::create_array(int name, int ndims, const int64_t* shape, int dtype, bool zero,
                           Array** out) {
     if (ndims < 1 || ndims > kMaxDims) return fail(CN_ERR_INVALID_ARGUMENT, "array rank must be 1..3");
-    if (!dtype_valid(dtype)) return fail(CN_ERR_BAD_DTYPE, "bad dtype code");
+    if (!dtype_storable(dtype)) return fail(CN_ERR_BAD_DTYPE, "bad dtype code");
     for (int d = 0; d < ndims; ++d)
         if (shape[d] < 0) return fail(CN_ERR_INVALID_ARGUMENT, "negative extent");
     Array* old = find(name);
@@ -780,13 +780,16 @@ int Context::execute_node(const Dag& dag, size_t* index) {
     if (node.roots.size() == 1 && node.roots[0]->opcode == OP_SET_REGION && node.roots[0]->operands.size() == 2) {
         const AstNode& r = *node.roots[0];
         const Operand& rhs = r.operands[1];
-        if (!rhs.is_ref && rhs.leaf && r.operands[0].leaf && !rhs.leaf->is_scalar && !rhs.leaf->is_broadcast) {
+        // storage types have no generated kernels: every assignment from an array is a copy
+        const Array* ta = r.operands[0].leaf ? find(r.operands[0].leaf->result_name) : nullptr;
+        const bool stored = ta && !dtype_valid(ta->dtype);
+        if (!rhs.is_ref && rhs.leaf && r.operands[0].leaf && !rhs.leaf->is_scalar && (!rhs.leaf->is_broadcast || stored)) {
             const AstNode& tl = *r.operands[0].leaf;
             const Region sreg = rhs.region.is_global ? Region::full(rhs.leaf->ndims, rhs.leaf->shape) : rhs.region;
             const Region treg = r.region.is_global ? Region::full(tl.ndims, tl.shape) : r.region;
             bool same = sreg.ndims == treg.ndims;
             for (int d = 0; same && d < sreg.ndims; ++d) same = sreg.extent(d) == treg.extent(d);
-            if (!same && sreg.size() > 1) {
+            if ((!same && sreg.size() > 1) || stored) {
                 ++*index;
                 return execute_cross_set_region(r);
             }
@@ -953,6 +956,11 @@ int Context::execute_node(const Dag& dag, size_t* index) {
             case OP_RANDU: last = execute_randu(*r); break;
             case OP_DIAG: last = execute_diag(*r); break;
             case OP_TILE: last = execute_tile(*r); break;
+            case OP_RMS_NORM: last = execute_rms_norm(node); break;
+            case OP_CAUSAL_CONV: last = execute_causal_conv(node); break;
+            case OP_SELECTIVE_SCAN: last = execute_selective_scan(node); break;
+            case OP_SAMPLE: last = execute_sample(node); break;
+            case OP_CONVERT: last = execute_convert(node); break;
             case OP_MATMATMUL:
             case OP_GET_REGION:
                 return fail(CN_ERR_UNSUPPORTED, "opcode " + std::to_string(r->opcode) +

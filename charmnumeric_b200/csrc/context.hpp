@@ -9,6 +9,7 @@
 #include <cuda.h>
 #include <cuda_runtime.h>
 
+#include <initializer_list>
 #include <map>
 #include <string>
 #include <unordered_map>
@@ -145,6 +146,8 @@ public:
     int put_local(int name, int ndims, const int64_t* shape, int dtype, int64_t capacity, const void* host_slab);
     int execute_single_node(const char* blob, int64_t size);
     int put(int name, int ndims, const int64_t* shape, int dtype, const void* host);
+    int put_device(int name, int ndims, const int64_t* shape, int dtype, const void* data, cudaStream_t stream);
+    int device_array(int name, void** data, void** stream);
     int delete_array(int name);
     int synchronize();
     int compile_group(const char* blob, int64_t size, uint64_t* handle);
@@ -231,6 +234,17 @@ private:
     int execute_cross_set_region(const AstNode& root);
     int execute_tile(const AstNode& root);
     int execute_create(const AstNode& root);
+    // sequence operators (sequence.cpp)
+    int execute_rms_norm(const DagNode& node);
+    int execute_causal_conv(const DagNode& node);
+    int execute_selective_scan(const DagNode& node);
+    int execute_sample(const DagNode& node);
+    int execute_convert(const DagNode& node);
+    struct SeqArg;
+    int seq_arg(const DagNode& node, size_t i, SeqArg* out);
+    int seq_result(const DagNode& node, size_t i, int ndims, const int64_t* shape, int dtype, Array** out);
+    int seq_whole(std::initializer_list<SeqArg*> args);
+    int seq_rows(const Array& x, std::initializer_list<const Array*> operands, std::initializer_list<const Array*> results);
     int try_plain_fill(const DagNode& node, bool* done);
     int exchange_halo(Array* a, cudaStream_t st);
     int fetch_operand_rows(Array* x, const struct Lattice& anchor, int64_t anchor_n0, const struct Lattice& lv, char** data,

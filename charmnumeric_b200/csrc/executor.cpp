@@ -1123,6 +1123,7 @@ int Context::execute_reduce(const AstNode& r) {
         if (x->dtype != y->dtype) return fail(CN_ERR_BAD_DTYPE, "dot operands have different dtypes");
     }
     const int dtype = x->dtype;
+    if (!dtype_valid(dtype)) return fail(CN_ERR_BAD_DTYPE, "reductions of float16 and int8 arrays are not supported; convert them first");
     const int64_t n = x->local_elems();
     const void* px = x->buf.data;
     const void* py = y ? y->buf.data : nullptr;
@@ -1155,6 +1156,7 @@ int Context::execute_matmul(const AstNode& r) {
     const bool column = x->ndims == 2 && x->shape[1] == 1;
     if (x->ndims != 1 && !column) return fail(CN_ERR_UNSUPPORTED, "matvec needs a 1-D vector or an (n, 1) column");
     if (A->dtype != x->dtype) return fail(CN_ERR_BAD_DTYPE, "matvec operands have different dtypes");
+    if (!dtype_valid(A->dtype)) return fail(CN_ERR_BAD_DTYPE, "matvec of float16 and int8 arrays is not supported; convert them first");
     if (!ra.unit_step() || !rx.unit_step()) return fail(CN_ERR_UNSUPPORTED, "matvec on stepped views is not supported");
     const int64_t rows = ra.extent(0), cols = ra.extent(1);
     if (cols != rx.extent(0)) return fail(CN_ERR_SHAPE_MISMATCH, "matrix columns differ from vector length");
@@ -1477,6 +1479,7 @@ int Context::execute_randu(const AstNode& r) {
         v[i] = op.leaf->scalar;
     }
     if (v[0] < 0 || v[0] > 9007199254740992.0) return fail(CN_ERR_INVALID_ARGUMENT, "RANDU seed must be an integer in [0, 2^53]");
+    if (!dtype_valid(r.dtype)) return fail(CN_ERR_BAD_DTYPE, "RANDU makes float32, float64, int32 and int64 arrays");
     Array* x = nullptr;
     int rc = create_array(r.result_name, r.ndims, r.shape, r.dtype, false, &x);
     if (rc) return rc;
@@ -1657,6 +1660,48 @@ int Context::put(int name, int ndims, const int64_t* shape, int dtype, const voi
         stats_.bytes_h2d += bytes;
     }
     x->mark_written();
+    return CN_OK;
+}
+
+// A whole array from device memory of another library.  `stream` is the stream its values were
+// made on: the copy waits for that stream, and that stream waits for the copy, so that the owner
+// may release or overwrite its memory in stream order as soon as this returns.
+int Context::put_device(int name, int ndims, const int64_t* shape, int dtype, const void* data, cudaStream_t stream) {
+    if (!initialised_) return fail(CN_ERR_NO_DEVICE, "context not initialised");
+    cudaSetDevice(device_);
+    cudaPointerAttributes at;
+    if (!data || cudaPointerGetAttributes(&at, data) != cudaSuccess ||
+        (at.type != cudaMemoryTypeDevice && at.type != cudaMemoryTypeManaged) ||
+        (at.type == cudaMemoryTypeDevice && at.device != device_)) {
+        cudaGetLastError();
+        return fail(CN_ERR_INVALID_ARGUMENT, "put_device: not memory of this context's GPU");
+    }
+    Array* x = nullptr;
+    int rc = create_array(name, ndims, shape, dtype, false, &x);
+    if (rc) return rc;
+    const size_t esz = dtype_size(dtype);
+    const size_t bytes = (size_t)x->local_elems() * esz;
+    x->mark_written();
+    if (!bytes) return CN_OK;
+    const char* src = (const char*)data + (size_t)x->row_begin * x->unit * esz;
+    cudaEvent_t ev = nullptr;
+    if ((rc = cuda_fail(cudaEventCreateWithFlags(&ev, cudaEventDisableTiming), "event"))) return rc;
+    cudaError_t e = cudaEventRecord(ev, stream);
+    if (e == cudaSuccess) e = cudaStreamWaitEvent(stream_, ev, 0);
+    if (e == cudaSuccess) e = cudaMemcpyAsync(x->buf.data, src, bytes, cudaMemcpyDeviceToDevice, stream_);
+    if (e == cudaSuccess) e = cudaEventRecord(ev, stream_);
+    if (e == cudaSuccess) e = cudaStreamWaitEvent(stream, ev, 0);
+    cudaEventDestroy(ev);
+    return cuda_fail(e, "put_device copy");
+}
+
+// Where this rank's rows of an array are, and the stream that the context's work runs on.
+int Context::device_array(int name, void** data, void** stream) {
+    if (!initialised_) return fail(CN_ERR_NO_DEVICE, "context not initialised");
+    Array* x = find(name);
+    if (!x) return fail(CN_ERR_UNKNOWN_ARRAY, "device_array: unknown array " + std::to_string(name));
+    if (data) *data = x->buf.data;
+    if (stream) *stream = (void*)stream_;
     return CN_OK;
 }
 

@@ -62,5 +62,6 @@ extern const char* const kDeviceHeaderText;
 extern const char* const kExpTableText;
 // Digest of the sources of the kernels built ahead of time (matvec, dot / sum, halo copies).
 extern const char* const kAotSourceDigest;
+extern const char* const kSequenceSourceDigest;
 
 }  // namespace cn

@@ -120,7 +120,7 @@ std::unique_ptr<AstNode> read_ast(Reader& r, int depth) {
     read_region(r, &n->region);
     int nops = r.i32();
     if (!r.ok) return n;
-    if (nops < 0 || nops > 8) {
+    if (nops < 0 || nops > 16) {
         r.fail("operand count out of range");
         return n;
     }

@@ -32,11 +32,13 @@ class ArrayOperation:
     """Opcode values of the wire protocol (charmnumeric.py:139-150) plus additions."""
     add, sub, mul, div, matmul, tanh, exp, tile, reduce, matmatmul, diag = range(11)
     sqrt, abs, sum, randu = 11, 12, 13, 14
+    rms_norm, causal_conv, selective_scan, sample, convert = 15, 16, 17, 18, 19
 
 
 class DType:
     """Element type encoding shared with the wire protocol (charmnumeric.py:34-75)."""
     FLOAT32, FLOAT64, INT32, INT64 = 0, 1, 2, 3
+    FLOAT16, INT8 = 4, 5  # storage types: no arithmetic (additions)
 
     @staticmethod
     def from_numpy(dt):
@@ -70,9 +72,21 @@ def _normalize_dtype(dtype):
         return _DEFAULT_DTYPE
     dt = np.dtype(dtype)
     if dt not in WIRE_DTYPES:
-        raise TypeError("charmnumeric only supports float32, float64, int32, and int64; "
-                        f"got {dt}")
+        raise TypeError("charmnumeric only supports float32, float64, int32, and int64, and float16 "
+                        f"and int8 as storage types; got {dt}")
     return dt
+
+
+def _is_storage(dtype):
+    return dtype in (np.dtype("float16"), np.dtype("int8"))
+
+
+def _arithmetic(*arrays):
+    """float16 and int8 arrays can be made, filled, assigned, converted and given to the operators
+    of sequence models; nothing is computed with them directly."""
+    for a in arrays:
+        if isinstance(a, _ArrayOps) and _is_storage(a.dtype):
+            raise TypeError(f"{a.dtype} is a storage type: convert the array with astype first")
 
 
 def _normalize_shape(shape):
@@ -114,7 +128,7 @@ def _size(shape):
 
 class _Info:
     """Identity of one backend array; op records keep these, never the user objects."""
-    __slots__ = ("name", "shape", "dtype", "alive", "materialised", "__weakref__")
+    __slots__ = ("name", "shape", "dtype", "alive", "materialised", "pins", "__weakref__")
 
     def __init__(self, name, shape, dtype):
         self.name = name
@@ -122,13 +136,14 @@ class _Info:
         self.dtype = dtype
         self.alive = True          # a user-facing Array / ArrayView still refers to it
         self.materialised = False  # exists in the backend's array table
+        self.pins = 0              # recorded steps that use the array
 
 
 class _Op:
     __slots__ = ("kind", "opcode", "result", "operands", "region", "payload")
 
     def __init__(self, kind, opcode=None, result=None, operands=(), region=None, payload=None):
-        self.kind = kind          # "ew", "set", "xset" (cross-dimension assignment), "create", "reduce", "sum", "matmul", "diag", "tile", "randu", "put"
+        self.kind = kind          # "ew", "set", "xset" (cross-dimension assignment), "create", "reduce", "sum", "matmul", "diag", "tile", "randu", "put", "fill", "seq" (an operator of sequence models; payload: the _Info of every result)
         self.opcode = opcode
         self.result = result      # _Info
         self.operands = list(operands)  # (_Info, Region | None) or python scalar
@@ -178,7 +193,7 @@ def _record(op):
 
 def _retire(info):
     info.alive = False
-    if info.materialised:
+    if info.materialised and not info.pins:
         _state.dead.append(info.name)
 
 
@@ -333,9 +348,13 @@ class _ArrayOps:
         self[...] = value
 
     def astype(self, dtype, copy=True):
-        if _normalize_dtype(dtype) != self.dtype:
-            raise NotImplementedError(
-                "dtype conversion for existing charmnumeric arrays is not implemented yet")
+        """The values in another type: rounded to the nearest into a floating-point type, as C
+        converts them into an integer type (values outside of its range are undefined)."""
+        dtype = _normalize_dtype(dtype)
+        if dtype != self.dtype:
+            out = _new_array(self.shape, dtype)
+            _record(_Op("seq", wire.OP_CONVERT, out._info, [_whole(self)._operand(), None, 0], payload=[out._info]))
+            return out
         return self.copy() if copy else self
 
     def __getitem__(self, key):
@@ -349,6 +368,20 @@ class _ArrayOps:
         if self._region is not None:
             region = _compose(self._region, region)
         rhs = _coerce_assignment(rhs, region.shape(), self.dtype)
+        if _is_storage(self.dtype) or (isinstance(rhs, _ArrayOps) and _is_storage(rhs.dtype)):
+            # no generated kernel takes these: a fill or a copy, its own node
+            if not isinstance(rhs, _ArrayOps):
+                _record(_Op("fill", wire.OP_SET_REGION, self._info, [rhs], region=region))
+                return
+            if rhs.dtype != self.dtype:
+                raise TypeError(f"cannot assign {rhs.dtype} to {self.dtype}: convert it with astype first")
+            if [d for d in rhs.shape if d != 1] != [d for d in region.shape() if d != 1]:
+                raise ValueError(f"could not broadcast input from shape {rhs.shape} "
+                                 f"into shape {region.shape()}")
+            if rhs._info is self._info:
+                rhs = rhs.copy()
+            _record(_Op("xset", wire.OP_SET_REGION, self._info, [rhs._operand()], region=region))
+            return
         if isinstance(rhs, _ArrayOps):
             if tuple(rhs.shape) != tuple(region.shape()) and rhs.size != 1:
                 # the same elements with the singleton dimensions elsewhere (`A[i, :] = v`,
@@ -390,6 +423,11 @@ class Array(_ArrayOps):
         execute(interface)
         data = interface.get(self.ndims, self.name, self.size, dtype=self.dtype)
         return data.reshape(self.shape)
+
+    def device_view(self, interface):
+        """The array's memory as an object with ``__cuda_array_interface__``."""
+        from .device import device_view
+        return device_view(self, interface)
 
 
 class ArrayView(_ArrayOps):
@@ -467,6 +505,7 @@ def _result_dtype(a, b):
 
 def _binary(opcode, a, b):
     a, b = _coerce_operand(a), _coerce_operand(b)
+    _arithmetic(a, b)
     out = _new_array(_result_shape(a, b), _result_dtype(a, b))
     operands = [x._operand() if isinstance(x, _ArrayOps) else x for x in (a, b)]
     _record(_Op("ew", opcode, out._info, operands))
@@ -475,6 +514,7 @@ def _binary(opcode, a, b):
 
 def _unary(opcode, x):
     x = asarray(x)
+    _arithmetic(x)
     out = _new_array(x.shape, x.dtype)
     _record(_Op("ew", opcode, out._info, [x._operand()]))
     return out
@@ -489,6 +529,7 @@ def _matmul(a, b):
     b = _coerce_operand(b)
     if not isinstance(b, _ArrayOps):
         raise ValueError("matmul does not support scalar operands")
+    _arithmetic(a, b)
     if a.ndims == b.ndims and (a.ndims == 1 or tuple(a.shape) == tuple(b.shape)) and \
             not (a.ndims == 2 and b.ndims == 2):
         if tuple(a.shape) != tuple(b.shape):
@@ -507,6 +548,7 @@ def _matmul(a, b):
 def _matvec(mat, vec):
     if not isinstance(vec, _ArrayOps):
         raise ValueError("matvec requires an Array vector")
+    _arithmetic(mat, vec)
     # a column vector (n, 1) has the memory layout and the partition of a 1-D vector of n
     column = vec.ndims == 2 and vec.shape[1] == 1
     if mat.ndims != 2 or not (vec.ndims == 1 or column):
@@ -560,6 +602,7 @@ def diag(v, k=0):
 def dot2d(a, b):
     """dot of two same-shaped arrays of any rank (the reference accepts 1-D only)."""
     a, b = _whole(asarray(a)), _whole(asarray(b))
+    _arithmetic(a, b)
     if tuple(a.shape) != tuple(b.shape):
         raise ValueError(f"Shape mismatch for dot product: {a.shape} vs {b.shape}")
     out = _new_array((1,), _result_dtype(a, b))
@@ -570,6 +613,7 @@ def dot2d(a, b):
 def sum_all(x):
     """Sum of all elements -> size-1 array (an addition; fuses behind the expression)."""
     x = asarray(x)
+    _arithmetic(x)
     out = _new_array((1,), x.dtype)
     _record(_Op("sum", wire.OP_SUM, out._info, [x._operand()]))
     return out
@@ -689,6 +733,8 @@ def uniform(shape, seed=0, low=0.0, high=1.0, dtype=_DEFAULT_DTYPE):
     """Seeded uniform array in [low, high): element with row-major index g depends only on
     (seed, g), whatever the number of GPUs.  (The reference's random.randn returns zeros,
     charmnumeric/random.py:4-5.)"""
+    if _is_storage(_normalize_dtype(dtype)):
+        raise TypeError("uniform makes float32, float64, int32 and int64 arrays; convert them with astype")
     out = _new_array(_normalize_shape(shape), _normalize_dtype(dtype))
     _record(_Op("randu", wire.OP_RANDU, out._info, [int(seed), float(low), float(high)]))
     return out
@@ -942,10 +988,23 @@ def _single_node(op):
         root = wire.Ast(res.name, wire.OP_DIAG, shape=res.shape, dtype=dt,
                         operands=[(_leaf(i), r) for i, r in op.operands]
                         + [(wire.scalar(float(op.payload)), None)])
-    elif op.kind == "xset":
-        src, sreg = op.operands[0]
+    elif op.kind == "seq":
+        # the operands, with a literal in the place of one that is left out, and one more root
+        # for every further result
+        operands = [(_leaf(o[0]), o[1]) if isinstance(o, tuple) else (wire.scalar(0.0 if o is None else float(o)), None)
+                    for o in op.operands]
+        roots = [wire.Ast(res.name, op.opcode, shape=res.shape, dtype=dt, operands=operands)]
+        roots += [wire.Ast(r.name, wire.OP_NOOP, shape=r.shape, dtype=WIRE_DTYPES[r.dtype]) for r in op.payload[1:]]
+        for r in op.payload:
+            r.materialised = True
+        node = wire.Node(_state.next_node, roots, fusible=False)
+        _state.next_node += 1
+        return node
+    elif op.kind in ("xset", "fill"):
+        rhs = op.operands[0]
+        rhs = (_leaf(rhs[0]), rhs[1]) if op.kind == "xset" else (wire.scalar(rhs, dt), None)
         root = wire.Ast(_state.new_name(), wire.OP_SET_REGION, shape=tuple(op.region.shape()), dtype=dt,
-                        region=op.region, operands=[(_leaf(res), None), (_leaf(src), sreg)])
+                        region=op.region, operands=[(_leaf(res), None), rhs])
         node = wire.Node(_state.next_node, [root], fusible=False)
         _state.next_node += 1
         return node
@@ -1001,7 +1060,7 @@ def build_nodes(ops):
         for op in seg_ops:
             for info, _ in _op_views(op):
                 readers.setdefault(info.name, set()).add(si)
-            if op.kind in ("set", "xset"):
+            if op.kind in ("set", "xset", "fill"):
                 # the target of an assignment has to exist as an array, even when the program
                 # drops its last handle on it before the batch is built
                 readers.setdefault(op.result.name, set()).add(si)
@@ -1053,8 +1112,9 @@ def execute(interface, mirror=None):
     dead = list(_state.dead)
     _state.dead.clear()
     for op in ops:
-        res = op.result
-        if res is not None and op.kind not in ("set", "xset") and res.materialised and not res.alive \
-                and res.name not in dead:
-            dead.append(res.name)
+        if op.kind in ("set", "xset", "fill"):
+            continue
+        for res in op.payload if op.kind == "seq" else [op.result]:
+            if res is not None and res.materialised and not res.alive and not res.pins and res.name not in dead:
+                dead.append(res.name)
     flush(dead)

@@ -23,9 +23,12 @@ OP_ADD, OP_SUB, OP_MUL, OP_DIV, OP_MATMUL, OP_TANH, OP_EXP = 0, 1, 2, 3, 4, 5, 6
 OP_TILE, OP_REDUCE, OP_MATMATMUL, OP_DIAG = 7, 8, 9, 10
 # additions of this backend
 OP_SQRT, OP_ABS, OP_SUM, OP_RANDU = 11, 12, 13, 14
+OP_RMS_NORM, OP_CAUSAL_CONV, OP_SELECTIVE_SCAN, OP_SAMPLE, OP_CONVERT = 15, 16, 17, 18, 19
 
 # dtype codes: charmnumeric/charmnumeric.py:37-40
 F32, F64, I32, I64 = 0, 1, 2, 3
+# storage types, additions of this backend
+F16, I8 = 4, 5
 
 
 class Region:

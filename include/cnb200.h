@@ -46,11 +46,34 @@ enum {
     CN_OP_NOOP = -1, CN_OP_ADD = 0, CN_OP_SUB = 1, CN_OP_MUL = 2, CN_OP_DIV = 3,
     CN_OP_MATMUL = 4, CN_OP_TANH = 5, CN_OP_EXP = 6, CN_OP_TILE = 7, CN_OP_REDUCE = 8,
     CN_OP_MATMATMUL = 9, CN_OP_DIAG = 10,
-    CN_OP_SQRT = 11, CN_OP_ABS = 12, CN_OP_SUM = 13, CN_OP_RANDU = 14
+    CN_OP_SQRT = 11, CN_OP_ABS = 12, CN_OP_SUM = 13, CN_OP_RANDU = 14,
+    /* operators of sequence models.  One non-fusible node each: root 0 has the operands in the
+     * order given, all of them whole arrays (a literal scalar leaf in the place of one that is left
+     * out), and a NOOP root behind it names every further result.  T is float16, float32 or
+     * float64, acc is float32 (float64 where T is).
+     * RMS_NORM (x T (.., n), weight T (n), residual T (.., n), literal eps, literal group)
+     *   -> y T, or with group > 0 int8 codes, scales acc (.., ceil(n / group)); with a residual
+     *   also x + residual T.
+     * CAUSAL_CONV (x T (b, t, d), weight T (d, k), bias T (d), state T (b, k-1, d), lengths int32
+     *   (b), literal activation: 0 none, 1 silu) -> y T (b, t, d), state T (b, k-1, d); 2 <= k <= 8.
+     * SELECTIVE_SCAN (x T (b, t, d), delta T (b, t, d), A acc (d, n), B T (b, t, g n), C T (b, t,
+     *   g n), D acc (d), z T (b, t, d), delta_bias acc (d), state acc (b, d, n), lengths int32 (b),
+     *   literal softplus 0/1) -> y T (b, t, d), state acc (b, d, n); n <= 256.
+     *   The state result of either may be the state operand itself (updated in place).
+     * SAMPLE (logits T (rows, v) or (v), u float32/float64 (rows), and temperature, top_k, top_p,
+     *   min_p, each a literal or an array (rows), top_k int32) -> token int32 (rows), log
+     *   probability acc (rows).
+     * CONVERT (x, scales, literal group) -> the values in the root's dtype; with scales x holds
+     *   int8 codes and the values are code * scale. */
+    CN_OP_RMS_NORM = 15, CN_OP_CAUSAL_CONV = 16, CN_OP_SELECTIVE_SCAN = 17, CN_OP_SAMPLE = 18,
+    CN_OP_CONVERT = 19
 };
 
-/* dtype codes: charmnumeric/charmnumeric.py:37-40 */
-enum { CN_DTYPE_F32 = 0, CN_DTYPE_F64 = 1, CN_DTYPE_I32 = 2, CN_DTYPE_I64 = 3 };
+/* dtype codes: charmnumeric/charmnumeric.py:37-40.  F16 and I8 are storage types (additions): such
+ * arrays can be created, filled, assigned, converted and moved, and the operators of sequence
+ * models take them; arithmetic on them returns CN_STATUS_BAD_DTYPE. */
+enum { CN_DTYPE_F32 = 0, CN_DTYPE_F64 = 1, CN_DTYPE_I32 = 2, CN_DTYPE_I64 = 3,
+       CN_DTYPE_F16 = 4, CN_DTYPE_I8 = 5 };
 
 int cn_version(void);
 const char* cn_status_string(int status);
@@ -99,6 +122,19 @@ int cn_get_local(cn_context* ctx, int name, int64_t* row_begin, int64_t* row_end
  * (charmnumeric/charmnumeric.py:863-878). */
 int cn_put(cn_context* ctx, int name, int ndims, const int64_t* shape, int dtype,
            const void* host);
+
+/* The same from device memory of this context's GPU that another library owns (row-major, the
+ * whole array; each rank copies its own slab).  `stream` is the cudaStream_t its values were
+ * made on (NULL: the default stream): the copy waits for that stream, and that stream waits for
+ * the copy.  Memory of another GPU or of the host: CN_STATUS_INVALID_ARGUMENT. */
+int cn_put_device(cn_context* ctx, int name, int ndims, const int64_t* shape, int dtype,
+                  const void* data, void* stream);
+/* Device address of this rank's rows of an array (dense, row-major) and the stream that the
+ * context's work runs on, for another library to read the values in place.  The address stays
+ * until the array is deleted, created with another shape, or assigned in place by a stencil sweep
+ * or a prompt's state update, which write a second buffer and exchange the two. */
+int cn_device_array(cn_context* ctx, int name, void** data, void** stream);
+
 
 /* The slab-wise counterpart of cn_put: `host_slab` holds only the rows this rank owns
  * (cn_partition of shape[0]), `capacity` its length in elements.  No counterpart in the

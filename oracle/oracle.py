@@ -24,6 +24,8 @@ from pathlib import Path
 
 import numpy as np
 
+from . import sequence
+
 _HERE = Path(__file__).resolve().parent
 _LIB = _HERE / "libcn_oracle.so"
 
@@ -31,8 +33,9 @@ OP_COPY, OP_SET_REGION, OP_CREATE, OP_NOOP = -5, -4, -2, -1
 OP_ADD, OP_SUB, OP_MUL, OP_DIV, OP_MATMUL, OP_TANH, OP_EXP, OP_REDUCE = 0, 1, 2, 3, 4, 5, 6, 8
 OP_TILE, OP_DIAG = 7, 10
 OP_SQRT, OP_ABS, OP_SUM, OP_RANDU = 11, 12, 13, 14
+OP_RMS_NORM, OP_CAUSAL_CONV, OP_SELECTIVE_SCAN, OP_SAMPLE, OP_CONVERT = 15, 16, 17, 18, 19
 NP_DTYPES = {0: np.dtype("float32"), 1: np.dtype("float64"), 2: np.dtype("int32"),
-             3: np.dtype("int64")}
+             3: np.dtype("int64"), 4: np.dtype("float16"), 5: np.dtype("int8")}
 
 
 def build(force=False):
@@ -287,6 +290,12 @@ class Oracle:
             elif op == OP_RANDU:
                 seed, lo, hi = (o[0].scalar for o in r.operands)
                 self.arrays[r.result_name] = randu(r.shape, int(seed), lo, hi, NP_DTYPES[r.dtype])
+            elif op in sequence.OPERATORS:
+                given = [o[0].scalar if o[0].is_scalar else self.arrays[o[0].result_name] for o in r.operands]
+                results = sequence.OPERATORS[op](*given, to=NP_DTYPES[r.dtype])
+                for root, value in zip(roots, results):
+                    self.arrays[root.result_name] = value
+                break
             else:
                 raise ValueError(f"oracle: opcode {op} not covered")
 
