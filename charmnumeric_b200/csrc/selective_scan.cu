@@ -99,10 +99,11 @@ __device__ __forceinline__ double gate(double z) { return z / (1.0 + exp(-z)); }
 // in pairs (p L + l) 2 + {0, 1}.  The time axis is walked in tiles of kSteps.  For each tile the block
 //   - computes (dt, dt x) of its channels and lays them, B and C into shared memory as floats, from
 //     values that were requested a tile ahead,
-//   - walks the steps: a lane's products of C and h are summed over its states, and every kGroup steps
-//     the L lanes of a channel add theirs up by halving exchanges, each ending with one step's sum,
-//   - adds D x, applies the gate and stores y, channels side by side.
-// One barrier a tile: two buffers alternate.
+//   - walks the steps; each lane lays the sum over its own states into shared memory,
+//   - adds up the lanes of a channel and D x, applies the gate and stores y, channels side by side.
+// One barrier a tile: two buffers alternate.  Sums through shared memory cost a store a step, and
+// nothing waits for them; the halving exchanges between lanes that were here first took 3.5
+// instructions a step and their latency with them.
 //
 // Where there are too few channels to fill the GPU, the time axis is cut into chunks.  A first pass
 // (LOCAL) computes each chunk's states from zero and the sum S of its dt; the second enters a chunk with
@@ -117,26 +118,45 @@ struct ScanChunks {
     A* sums = nullptr;    // (b, count, d)
 };
 
+template <typename A> struct alignas(16) Four { Two<A> x, y; };
+
 template <typename A, int L, int N, bool LOCAL>
 struct ScanShared {
     static constexpr int kChannels = kThreads / L, kPairs = N / 2;
-    static constexpr int kPitch = kChannels + 32 / L;      // lanes of a warp store to different banks
     static constexpr int kTiles = LOCAL ? 1 : 2;
-    alignas(16) A step[2][kChannels][kSteps + 1][4];       // dt, dt, dt x, dt x
-    alignas(16) A b[2][kSteps / 2][kPairs][L][4];          // two steps' pairs
-    alignas(16) A c[kTiles][kSteps / 2][kPairs][L][4];
-    A y[kTiles][kSteps][kPitch];
+    Four<A> step[2][kChannels][kSteps + 1];                // (dt, dt), (dt x, dt x); one more against bank conflicts
+    Four<A> b[2][kSteps / 2][kPairs][L];                   // the pairs of two steps
+    Four<A> c[kTiles][kSteps / 2][kPairs][L];
+    alignas(16) A y[kTiles][kSteps][kThreads];             // every lane's sum over its states
 };
+
+// sum of the L lanes of a channel; the pieces are read in an order that keeps the banks apart
+template <int L, typename A>
+__device__ __forceinline__ A lanes_sum(const A* y, int slot) {
+    constexpr int V = 16 / sizeof(A) < L ? 16 / sizeof(A) : L, kPieces = L / V;
+    A t = 0;
+#pragma unroll
+    for (int k = 0; k < kPieces; ++k) {
+        const int piece = (k + slot * L / 32) % kPieces;
+        const Pack<A, V> v = *(const Pack<A, V>*)(y + slot * L + piece * V);
+        A s = v.v[0];
+#pragma unroll
+        for (int j = 1; j < V; ++j) s += v.v[j];
+        t += s;
+    }
+    return t;
+}
 
 template <typename T, int L, int N, bool LOCAL>
 __global__ void __launch_bounds__(kThreads) scan_kernel(SelectiveScanArgs a, ScanChunks<typename Acc<T>::type> ck, int blocks) {
     using A = typename Acc<T>::type;
     constexpr int kChannels = kThreads / L;
     constexpr int kPairs = N / 2;
-    constexpr int kGroup = L < 8 ? L : 8;
-    constexpr int kOwn = (kSteps * kChannels + kThreads - 1) / kThreads;
+    constexpr int kOwn = (kSteps * kChannels + kThreads - 1) / kThreads;     // values of x, delta, z a thread lays down
+    constexpr int kRows = kThreads / kChannels;                              // ... kRows steps apart
     constexpr int kStates = L * N;
     constexpr int kOwnB = (kSteps * kStates + kThreads - 1) / kThreads;
+    constexpr int kGroup = kPairs >= 4 ? 2 : 4;                              // steps whose exponentials are made together
     extern __shared__ __align__(16) unsigned char scan_shared[];
     auto& sh = *(ScanShared<A, L, N, LOCAL>*)scan_shared;
 
@@ -147,13 +167,8 @@ __global__ void __launch_bounds__(kThreads) scan_kernel(SelectiveScanArgs a, Sca
     const int64_t g = blk / per_blocks, c0 = g * per_group + blk % per_blocks * kChannels, c1 = (g + 1) * per_group;
     const int64_t end_all = a.lengths ? min(max((int64_t)a.lengths[b], (int64_t)0), a.t) : a.t;
     const int64_t t0 = blockIdx.y * ck.length;
-    const int64_t stop = min(t0 + ck.length, a.t), end = min(stop, end_all);     // end < t0: nothing to walk
+    const int64_t stop = min(t0 + ck.length, a.t), end = min(stop, end_all);     // end <= t0: nothing to walk
     const int64_t bn = (int64_t)a.groups * a.n;
-    const T* const xs = (const T*)a.x + b * a.t * a.d;
-    const T* const ds = (const T*)a.delta + b * a.t * a.d;
-    const T* const zs = a.z ? (const T*)a.z + b * a.t * a.d : nullptr;
-    const T* const bs = (const T*)a.B + b * a.t * bn + g * a.n;
-    const T* const cs = (const T*)a.C + b * a.t * bn + g * a.n;
 
     // a lane's states and decays
     const int64_t c = c0 + own;
@@ -181,45 +196,53 @@ __global__ void __launch_bounds__(kThreads) scan_kernel(SelectiveScanArgs a, Sca
         }
     }
 
-    // values of a tile that this thread lays down: requested early, used a tile later
-    T rx[kOwn], rd[kOwn], rz[kOwn], rb[kOwnB], rc[kOwnB];
-    A px[kOwn], pz[kOwn];       // the tile being walked: for the skip and the gate
-    A sum = 0;                  // LOCAL: dt summed over the chunk, for the channel of slot tid % kChannels
-    auto request = [&](int64_t from) {
+    // what this thread lays down: x, delta, z of one channel, kRows steps apart, and pieces of B and C
+    const int row = tid / kChannels, slot = tid % kChannels;
+    const int64_t ch = c0 + slot;
+    const bool mine = ch < c1 && row < kSteps;
+    const A bias = mine && a.delta_bias ? ((const A*)a.delta_bias)[ch] : A(0);
+    const A skip = mine && a.D ? ((const A*)a.D)[ch] : A(0);
+    const int64_t first = (b * a.t + t0 + row) * a.d + ch, stride = kRows * a.d, tile = kSteps * a.d;
+    const T *xs = (const T*)a.x + first, *ds = (const T*)a.delta + first, *zs = a.z ? (const T*)a.z + first : nullptr;
+    T* ys = (T*)a.y + first;
+    const T *bs = (const T*)a.B + (b * a.t + t0) * bn + g * a.n, *cs = (const T*)a.C + (b * a.t + t0) * bn + g * a.n;
+
+    T rx[kOwn], rd[kOwn], rz[kOwn], rb[kOwnB], rc[kOwnB];     // requested early, used a tile later
+    A px[kOwn], pz[kOwn];                                     // of the tile being walked: for the skip and the gate
+    A sum = 0;                                                // LOCAL: dt summed over the chunk
+    const T zero = narrow<T>(A(0));
+    auto request = [&](int live) {
 #pragma unroll
         for (int i = 0; i < kOwn; ++i) {
-            const int e = tid + i * kThreads;
-            const int64_t t = from + e / kChannels, ch = c0 + e % kChannels;
-            const bool on = t < end && ch < c1 && e < kSteps * kChannels;
-            const int64_t at = t * a.d + ch;
-            rx[i] = on ? xs[at] : narrow<T>(A(0));
-            rd[i] = on ? ds[at] : narrow<T>(A(0));
-            if (!LOCAL) rz[i] = on && zs ? zs[at] : narrow<T>(A(0));
+            const bool on = mine && row + i * kRows < live;
+            rx[i] = on ? xs[i * stride] : zero;
+            rd[i] = on ? ds[i * stride] : zero;
+            if (!LOCAL) rz[i] = on && a.z ? zs[i * stride] : zero;
         }
+        xs += tile;
+        ds += tile;
+        if (!LOCAL && a.z) zs += tile;
 #pragma unroll
         for (int i = 0; i < kOwnB; ++i) {
-            const int e = tid + i * kThreads, n = e % kStates;
-            const int64_t t = from + e / kStates;
-            const bool on = t < end && n < a.n && e < kSteps * kStates;
-            rb[i] = on ? bs[t * bn + n] : narrow<T>(A(0));
-            if (!LOCAL) rc[i] = on ? cs[t * bn + n] : narrow<T>(A(0));
+            const int e = tid + i * kThreads, n = e % kStates, s = e / kStates;
+            const bool on = s < live && n < a.n;
+            rb[i] = on ? bs[s * bn + n] : zero;
+            if (!LOCAL) rc[i] = on ? cs[s * bn + n] : zero;
         }
+        bs += kSteps * bn;
+        cs += kSteps * bn;
     };
-    auto lay = [&](int64_t from, int buf) {
+    auto lay = [&](int live, int buf) {
+        if (row < kSteps) {
 #pragma unroll
-        for (int i = 0; i < kOwn; ++i) {
-            const int e = tid + i * kThreads;
-            if (kSteps * kChannels % kThreads && e >= kSteps * kChannels) break;
-            const int s = e / kChannels, slot = e % kChannels;
-            const bool on = from + s < end && c0 + slot < c1;
-            A dt = widen(rd[i]) + (on && a.delta_bias ? ((const A*)a.delta_bias)[c0 + slot] : A(0));
-            if (a.softplus) dt = softplus(dt);
-            if (!on) dt = 0;
-            const A x = widen(rx[i]), dtx = dt * x;
-            A* const to = sh.step[buf][slot][s];
-            *(Two<A>*)to = {dt, dt};
-            *(Two<A>*)(to + 2) = {dtx, dtx};
-            if (LOCAL) sum += dt;
+            for (int i = 0; i < kOwn; ++i) {
+                A dt = widen(rd[i]) + bias;
+                if (a.softplus) dt = softplus(dt);
+                if (!mine || row + i * kRows >= live) dt = 0;
+                const A dtx = dt * widen(rx[i]);
+                sh.step[buf][slot][row + i * kRows] = {{dt, dt}, {dtx, dtx}};
+                if (LOCAL) sum += dt;
+            }
         }
 #pragma unroll
         for (int i = 0; i < kOwnB; ++i) {
@@ -227,8 +250,8 @@ __global__ void __launch_bounds__(kThreads) scan_kernel(SelectiveScanArgs a, Sca
             if (kSteps * kStates % kThreads && e >= kSteps * kStates) break;
             const int s = e / kStates, n = e % kStates;
             const int p = n / (2 * L), l = n % (2 * L) / 2, j = (s & 1) * 2 + (n & 1);
-            sh.b[buf][s / 2][p][l][j] = widen(rb[i]);
-            if (!LOCAL) sh.c[buf][s / 2][p][l][j] = widen(rc[i]);
+            ((A*)&sh.b[buf][s / 2][p][l])[j] = widen(rb[i]);
+            if (!LOCAL) ((A*)&sh.c[buf][s / 2][p][l])[j] = widen(rc[i]);
         }
     };
 
@@ -237,67 +260,42 @@ __global__ void __launch_bounds__(kThreads) scan_kernel(SelectiveScanArgs a, Sca
 #pragma unroll
         for (int s0 = 0; s0 < kSteps; s0 += kGroup) {
             if (!kWhole && s0 >= live) break;
-            A part[kGroup];
+            Two<A> e[kGroup][kPairs], term[kGroup][kPairs];
+            // all of the group's exponentials and terms, which wait for no state ...
 #pragma unroll
             for (int i = 0; i < kGroup; i += 2) {
-                Two<A> bb[kPairs][2], cc[kPairs][2];
+                const Four<A> u = sh.step[buf][own][s0 + i], v = sh.step[buf][own][s0 + i + 1];
 #pragma unroll
                 for (int p = 0; p < kPairs; ++p) {
-                    const A* q = sh.b[buf][(s0 + i) / 2][p][lane];
-                    const Pack<A, 16 / sizeof(A)>* v = (const Pack<A, 16 / sizeof(A)>*)q;
-                    Pack<A, 16 / sizeof(A)> w[sizeof(A) / 4];
-#pragma unroll
-                    for (int k = 0; k < (int)sizeof(A) / 4; ++k) w[k] = v[k];
-                    bb[p][0] = ((Two<A>*)w)[0];
-                    bb[p][1] = ((Two<A>*)w)[1];
-                    if (!LOCAL) {
-                        const Pack<A, 16 / sizeof(A)>* u = (const Pack<A, 16 / sizeof(A)>*)sh.c[buf][(s0 + i) / 2][p][lane];
-#pragma unroll
-                        for (int k = 0; k < (int)sizeof(A) / 4; ++k) w[k] = u[k];
-                        cc[p][0] = ((Two<A>*)w)[0];
-                        cc[p][1] = ((Two<A>*)w)[1];
-                    }
+                    const Four<A> bb = sh.b[buf][(s0 + i) / 2][p][lane];
+                    const Two<A> m0 = mul(u.x, decay[p]), m1 = mul(v.x, decay[p]);
+                    e[i][p] = {power(m0.x), power(m0.y)};
+                    e[i + 1][p] = {power(m1.x), power(m1.y)};
+                    term[i][p] = mul(u.y, bb.x);
+                    term[i + 1][p] = mul(v.y, bb.y);
                 }
+            }
+            // ... then the recurrence
 #pragma unroll
-                for (int k = 0; k < 2; ++k) {
-                    if (i + k >= kGroup) break;
-                    Pack<A, 16 / sizeof(A)> w[sizeof(A) / 4];
-                    const Pack<A, 16 / sizeof(A)>* v = (const Pack<A, 16 / sizeof(A)>*)sh.step[buf][own][s0 + i + k];
+            for (int i = 0; i < kGroup; i += 2) {
+                Two<A> y[2];
 #pragma unroll
-                    for (int r = 0; r < (int)sizeof(A) / 4; ++r) w[r] = v[r];
-                    const Two<A> dt = ((Two<A>*)w)[0], dtx = ((Two<A>*)w)[1];
-                    Two<A> y;
+                for (int p = 0; p < kPairs; ++p) {
+                    Four<A> cc;
+                    if (!LOCAL) cc = sh.c[buf][(s0 + i) / 2][p][lane];
 #pragma unroll
-                    for (int p = 0; p < kPairs; ++p) {
-                        const Two<A> m = mul(dt, decay[p]);
-                        const Two<A> e = {power(m.x), power(m.y)};
-                        const Two<A> next = fma(e, h[p], mul(dtx, bb[p][k]));
-                        // behind the end the step is left out: 0 times an infinite A is not 0
+                    for (int k = 0; k < 2; ++k) {
+                        const Two<A> next = fma(e[i + k][p], h[p], term[i + k][p]);
+                        // behind the end a step is left out: 0 times an infinite A is not 0
                         if (kWhole || s0 + i + k < live) h[p] = next;
-                        if (!LOCAL) y = p ? fma(cc[p][k], h[p], y) : mul(cc[p][k], h[p]);
+                        if (!LOCAL) y[k] = p ? fma(k ? cc.y : cc.x, h[p], y[k]) : mul(k ? cc.y : cc.x, h[p]);
                     }
-                    if (!LOCAL) part[i + k] = y.x + y.y;
+                }
+                if (!LOCAL) {
+                    sh.y[buf][s0 + i][tid] = y[0].x + y[0].y;
+                    sh.y[buf][s0 + i + 1][tid] = y[1].x + y[1].y;
                 }
             }
-            if (LOCAL) continue;
-            // lanes at distance o exchange halves; a lane ends with the sum of step lane / (L / kGroup)
-            int width = kGroup;
-#pragma unroll
-            for (int o = L / 2; o > 0; o >>= 1) {
-                if (width > 1) {
-                    width /= 2;
-                    const bool up = lane & o;
-#pragma unroll
-                    for (int i = 0; i < kGroup / 2; ++i) {
-                        if (i >= width) break;
-                        const A send = up ? part[i] : part[i + width], keep = up ? part[i + width] : part[i];
-                        part[i] = keep + __shfl_xor_sync(0xffffffffu, send, o);
-                    }
-                } else {
-                    part[0] += __shfl_xor_sync(0xffffffffu, part[0], o);
-                }
-            }
-            if (lane % (L / kGroup) == 0) sh.y[buf][s0 + lane / (L / kGroup)][own] = part[0];
         }
     };
 
@@ -310,40 +308,37 @@ __global__ void __launch_bounds__(kThreads) scan_kernel(SelectiveScanArgs a, Sca
     };
 
     if (t0 < end) {
-        request(t0);
-        lay(t0, 0);
+        int live = (int)min(end - t0, (int64_t)kSteps);
+        request(live);
+        lay(live, 0);
         keep();
         __syncthreads();
         int buf = 0;
         for (int64_t t = t0; t < end; t += kSteps, buf ^= 1) {
-            const bool more = t + kSteps < end;
-            if (more) request(t + kSteps);
-            const int live = (int)min(end - t, (int64_t)kSteps);
+            const int next = (int)min(max(end - t - kSteps, (int64_t)0), (int64_t)kSteps);
+            if (next) request(next);
             if (live == kSteps) walk(buf, live, std::true_type());
             else walk(buf, live, std::false_type());
-            if (more) lay(t + kSteps, buf ^ 1);
+            if (next) lay(next, buf ^ 1);
             __syncthreads();
             if (!LOCAL) {
 #pragma unroll
                 for (int i = 0; i < kOwn; ++i) {
-                    const int e = tid + i * kThreads;
-                    if (kSteps * kChannels % kThreads && e >= kSteps * kChannels) break;
-                    const int s = e / kChannels, slot = e % kChannels;
-                    const int64_t ch = c0 + slot;
-                    if (s >= live || ch >= c1) continue;
-                    A y = sh.y[buf][s][slot];
-                    if (a.D) y += ((const A*)a.D)[ch] * px[i];
-                    if (zs) y *= gate(pz[i]);
-                    ((T*)a.y)[(b * a.t + t + s) * a.d + ch] = narrow<T>(y);
+                    if (!mine || row + i * kRows >= live) continue;
+                    A y = lanes_sum<L>(sh.y[buf][row + i * kRows], slot) + skip * px[i];
+                    if (a.z) y *= gate(pz[i]);
+                    ys[i * stride] = narrow<T>(y);
                 }
+                ys += tile;
             }
-            if (more) keep();
+            if (next) keep();
+            live = next;
         }
     }
     if (LOCAL) {
-        // dt of a channel was summed by kThreads / kChannels threads: add them up in their order
+        // dt of a channel was summed by kRows threads: add them up in their order
         __syncthreads();
-        A* const part = &sh.step[0][0][0][0];
+        A* const part = (A*)&sh.step;
         part[tid] = sum;
         __syncthreads();
         if (tid < kChannels && c0 + tid < c1) {
@@ -353,9 +348,10 @@ __global__ void __launch_bounds__(kThreads) scan_kernel(SelectiveScanArgs a, Sca
         }
     } else {
         // rows behind the end of the sequence
-        for (int64_t e = tid; e < (stop - max(end, t0)) * kChannels; e += kThreads) {
-            const int64_t ch = c0 + e % kChannels, t = max(end, t0) + e / kChannels;
-            if (ch < c1) ((T*)a.y)[(b * a.t + t) * a.d + ch] = narrow<T>(A(0));
+        const int64_t from = max(end, t0);
+        for (int64_t e = tid; e < (stop - from) * kChannels; e += kThreads) {
+            const int64_t cc = c0 + e % kChannels;
+            if (cc < c1) ((T*)a.y)[(b * a.t + from + e / kChannels) * a.d + cc] = zero;
         }
         if ((int)blockIdx.y != ck.count - 1) return;
     }
