@@ -24,34 +24,27 @@ using namespace seq;
 
 namespace {
 
-constexpr int kThreads = 256;
-constexpr int kSteps = 16;      // time steps staged in shared memory at once
+constexpr int kThreads = 256, kHelpers = 256;
 
 // ---- arithmetic -------------------------------------------------------------------------------------
 
 // Two values side by side.  Floats are multiplied and added in pairs by one instruction each.
 template <typename A> struct alignas(2 * sizeof(A)) Two { A x, y; };
 
-__device__ __forceinline__ unsigned long long as_bits(Two<float> v) {
-    unsigned long long r;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(v.x), "f"(v.y));
-    return r;
-}
-__device__ __forceinline__ Two<float> as_two(unsigned long long r) {
-    Two<float> v;
-    asm("mov.b64 {%0, %1}, %2;" : "=f"(v.x), "=f"(v.y) : "l"(r));
-    return v;
-}
 __device__ __forceinline__ Two<float> mul(Two<float> a, Two<float> b) {
-    unsigned long long r;
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(as_bits(a)), "l"(as_bits(b)));
-    return as_two(r);
+    const float2 r = __fmul2_rn({a.x, a.y}, {b.x, b.y});
+    return {r.x, r.y};
 }
 __device__ __forceinline__ Two<float> fma(Two<float> a, Two<float> b, Two<float> c) {
-    unsigned long long r;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(as_bits(a)), "l"(as_bits(b)), "l"(as_bits(c)));
-    return as_two(r);
+    const float2 r = __ffma2_rn({a.x, a.y}, {b.x, b.y}, {c.x, c.y});
+    return {r.x, r.y};
 }
+__device__ __forceinline__ Two<float> add(Two<float> a, Two<float> b) {
+    const float2 r = __fadd2_rn({a.x, a.y}, {b.x, b.y});
+    return {r.x, r.y};
+}
+__device__ __forceinline__ Two<double> add(Two<double> a, Two<double> b) { return {a.x + b.x, a.y + b.y}; }
+template <typename A> __device__ __forceinline__ Two<A> both(A v) { return {v, v}; }
 __device__ __forceinline__ Two<double> mul(Two<double> a, Two<double> b) { return {a.x * b.x, a.y * b.y}; }
 __device__ __forceinline__ Two<double> fma(Two<double> a, Two<double> b, Two<double> c) {
     return {::fma(a.x, b.x, c.x), ::fma(a.y, b.y, c.y)};
@@ -88,283 +81,429 @@ __device__ __forceinline__ float softplus(float v) {
     p = fmaf(p, q, 1.0f / 3.0f);
     return fmaxf(v, 0.0f) + 2.0f * fmaf(p * q, s, s);
 }
+__device__ __forceinline__ Two<float> softplus(Two<float> v) {
+    const Two<float> e = {power(-1.4426950408889634f * fabsf(v.x)), power(-1.4426950408889634f * fabsf(v.y))};
+    const Two<float> u = add(e, both(2.0f));
+    const Two<float> s = mul(e, {reciprocal(u.x), reciprocal(u.y)}), q = mul(s, s);
+    Two<float> p = both(1.0f / 15.0f);
+    p = fma(p, q, both(1.0f / 13.0f));
+    p = fma(p, q, both(1.0f / 11.0f));
+    p = fma(p, q, both(1.0f / 9.0f));
+    p = fma(p, q, both(1.0f / 7.0f));
+    p = fma(p, q, both(1.0f / 5.0f));
+    p = fma(p, q, both(1.0f / 3.0f));
+    p = fma(mul(p, q), s, s);
+    return fma(p, both(2.0f), {fmaxf(v.x, 0.0f), fmaxf(v.y, 0.0f)});
+}
 __device__ __forceinline__ double softplus(double v) { return (v > 0 ? v : 0.0) + log1p(exp(-fabs(v))); }
+__device__ __forceinline__ Two<double> softplus(Two<double> v) { return {softplus(v.x), softplus(v.y)}; }
 
 __device__ __forceinline__ float gate(float z) { return z * reciprocal(1.0f + power(-1.4426950408889634f * z)); }
 __device__ __forceinline__ double gate(double z) { return z / (1.0 + exp(-z)); }
+__device__ __forceinline__ Two<float> gate(Two<float> z) {
+    const Two<float> m = mul(z, both(-1.4426950408889634f));
+    const Two<float> u = add({power(m.x), power(m.y)}, both(1.0f));
+    return mul(z, {reciprocal(u.x), reciprocal(u.y)});
+}
+__device__ __forceinline__ Two<double> gate(Two<double> z) { return {gate(z.x), gate(z.y)}; }
 
 // ---- prompts ------------------------------------------------------------------------------------------
 //
-// A block has kThreads / L channels of one sequence and group, L lanes for each; a lane has N states,
-// in pairs (p L + l) 2 + {0, 1}.  The time axis is walked in tiles of kSteps.  For each tile the block
-//   - computes (dt, dt x) of its channels and lays them, B and C into shared memory as floats, from
-//     values that were requested a tile ahead,
-//   - walks the steps; each lane lays the sum over its own states into shared memory,
-//   - adds up the lanes of a channel and D x, applies the gate and stores y, channels side by side.
-// One barrier a tile: two buffers alternate.  Sums through shared memory cost a store a step, and
-// nothing waits for them; the halving exchanges between lanes that were here first took 3.5
-// instructions a step and their latency with them.
+// A block has kThreads / L channels of one sequence and group.  The time axis is walked in tiles of S
+// steps, by two halves of the block that work side by side, one barrier a tile:
+//   - kThreads walkers, L for each channel; a walker has N states, in pairs (p L + l) 2 + {0, 1}, and
+//     sums C h over its own states at every step, which goes through shared memory.  The exponentials
+//     of the next steps are made before the recurrence of the present ones, which waits for them else;
+//   - kThreads helpers, which copy tiles into a ring in shared memory some tiles ahead (cp.async), lay
+//     (dt, dt x), B and C of the next tile down as floats, and finish the tile before: they add up the
+//     lanes of each channel and D x, apply the gate and store y.
+// The laid-down values and the sums have two buffers each, which alternate.
 //
 // Where there are too few channels to fill the GPU, the time axis is cut into chunks.  A first pass
-// (LOCAL) computes each chunk's states from zero and the sum S of its dt; the second enters a chunk with
-//   h <- exp(A S_k) h + local_k   over the chunks k before it
+// (LOCAL) computes each chunk's states from zero and the sum of its dt; the second enters a chunk with
+//   h <- exp(A sum_k) h + local_k   over the chunks k before it
 // which costs every exponential twice.
 
 template <typename A>
 struct ScanChunks {
-    int64_t length = 0;   // steps of a chunk, a multiple of kSteps
+    int64_t length = 0;   // steps of a chunk, whole tiles
     int count = 1;
     A* local = nullptr;   // (b, count, d, n)
     A* sums = nullptr;    // (b, count, d)
 };
 
-template <typename A> struct alignas(16) Four { Two<A> x, y; };
-
-template <typename A, int L, int N, bool LOCAL>
+template <typename T, int L, int N, int S, bool LOCAL>
 struct ScanShared {
-    static constexpr int kChannels = kThreads / L, kPairs = N / 2;
-    static constexpr int kTiles = LOCAL ? 1 : 2;
-    Four<A> step[2][kChannels][kSteps + 1];                // (dt, dt), (dt x, dt x); one more against bank conflicts
-    Four<A> b[2][kSteps / 2][kPairs][L];                   // the pairs of two steps
-    Four<A> c[kTiles][kSteps / 2][kPairs][L];
-    alignas(16) A y[kTiles][kSteps][kThreads];             // every lane's sum over its states
+    using A = typename Acc<T>::type;
+    static constexpr int kChannels = kThreads / L, kPairs = N / 2, kStates = L * N;
+    // a ring row has room for the bytes between the 16-byte border before its first value and that value
+    static constexpr int kPitch = kThreads / 2 + 16;           // neighbouring steps in different banks
+    static constexpr int kRow = kChannels * (int)sizeof(T) + 16, kRowB = kStates * (int)sizeof(T) + 16;
+    struct Fixed {
+        alignas(16) A step[2][kChannels][S + 2][2];            // dt, dt x
+        alignas(16) T bc[2][S / 2][kPairs][L][8];              // a lane's pairs of B of two steps, and of C
+        alignas(16) A y[2][S][kPitch];                         // L / 2 sums of each channel
+    };
+    struct alignas(16) Stage {
+        unsigned char x[S][kRow], delta[S][kRow], z[S][kRow];
+        unsigned char b[S][kRowB], c[S][kRowB];
+    };
+    // tiles in the ring: the one to finish, the one that is walked, the one to lay down, and one or more
+    // on their way, as many as let two blocks share an SM (one block of the larger kinds)
+    static constexpr size_t kBudget = (sizeof(T) <= 4 && N == 2 ? 113 : 226) * 1024;
+    static constexpr int kFits = sizeof(Fixed) < kBudget ? (int)((kBudget - sizeof(Fixed)) / sizeof(Stage)) : 0;
+    static constexpr int kStages = kFits < 4 ? 4 : kFits > 8 ? 8 : kFits;
+    Fixed f;
+    Stage ring[kStages];
+    static_assert(sizeof(Fixed) + kStages * sizeof(Stage) <= 227 * 1024, "shared memory of an SM");
 };
 
-// sum of the L lanes of a channel; the pieces are read in an order that keeps the banks apart
-template <int L, typename A>
+// sum of K numbers of a channel; the pieces are read in an order that keeps the banks apart
+template <int K, typename A>
 __device__ __forceinline__ A lanes_sum(const A* y, int slot) {
-    constexpr int V = 16 / sizeof(A) < L ? 16 / sizeof(A) : L, kPieces = L / V;
+    constexpr int V = 16 / (int)sizeof(A) < K ? 16 / (int)sizeof(A) : K, kPieces = K / V;
     A t = 0;
 #pragma unroll
     for (int k = 0; k < kPieces; ++k) {
-        const int piece = (k + slot * L / 32) % kPieces;
-        const Pack<A, V> v = *(const Pack<A, V>*)(y + slot * L + piece * V);
+        const int piece = (k + slot * K / 32) % kPieces;
+        const Pack<A, V> v = *(const Pack<A, V>*)(y + slot * K + piece * V);
         A s = v.v[0];
 #pragma unroll
         for (int j = 1; j < V; ++j) s += v.v[j];
-        t += s;
+        t = k ? t + s : s;
     }
     return t;
 }
 
-template <typename T, int L, int N, bool LOCAL>
-__global__ void __launch_bounds__(kThreads) scan_kernel(SelectiveScanArgs a, ScanChunks<typename Acc<T>::type> ck, int blocks) {
-    using A = typename Acc<T>::type;
-    constexpr int kChannels = kThreads / L;
-    constexpr int kPairs = N / 2;
-    constexpr int kOwn = (kSteps * kChannels + kThreads - 1) / kThreads;     // values of x, delta, z a thread lays down
-    constexpr int kRows = kThreads / kChannels;                              // ... kRows steps apart
-    constexpr int kStates = L * N;
-    constexpr int kOwnB = (kSteps * kStates + kThreads - 1) / kThreads;
-    constexpr int kGroup = kPairs >= 4 ? 2 : 4;                              // steps whose exponentials are made together
-    extern __shared__ __align__(16) unsigned char scan_shared[];
-    auto& sh = *(ScanShared<A, L, N, LOCAL>*)scan_shared;
+template <int V, typename A>
+__device__ __forceinline__ Pack<A, V> load_shared(const A* p) {
+    // 16 bytes an access
+    constexpr int W = 16 / (int)sizeof(A);
+    Pack<A, V> r;
+#pragma unroll
+    for (int i = 0; i < V; i += W) *(Pack<A, W>*)&r.v[i] = *(const Pack<A, W>*)(p + i);
+    return r;
+}
 
-    const int tid = threadIdx.x, lane = tid & (L - 1), own = tid / L;
+// Rows are copied into the ring in pieces of 16 bytes where every row begins at a 16-byte border, else
+// of 8 (64-bit values) or 4: from the 4-byte border before a row's first value to the one behind its
+// last.  16-bit values of an odd place begin in the middle of a piece; the values around a row belong
+// to the array or to the room that every array has around it.
+template <typename T, int L, int N, int S, bool LOCAL>
+__global__ void __launch_bounds__(kThreads + kHelpers, sizeof(T) <= 4 && N == 2 ? 2 : 1) scan_kernel(SelectiveScanArgs a, ScanChunks<typename Acc<T>::type> ck, int blocks, int piece) {
+    using A = typename Acc<T>::type;
+    using Shared = ScanShared<T, L, N, S, LOCAL>;
+    constexpr int kChannels = Shared::kChannels, kPairs = Shared::kPairs, kStates = Shared::kStates, kStages = Shared::kStages;
+    constexpr int kAhead = kStages - 2;                                      // tiles requested ahead of the walked one
+    constexpr int kRows = kHelpers / kChannels;                              // a helper's steps are kRows apart
+    constexpr int kOwn = (S + kRows - 1) / kRows;
+    constexpr int kOwnB = (S * kStates + kHelpers - 1) / kHelpers;
+    constexpr int kGroup = kPairs >= 4 || sizeof(A) == 8 ? 2 : 4, kGroups = S / kGroup;   // steps whose exponentials are made together
+    constexpr int kMade = sizeof(A) == 8 ? 1 : 2;                            // groups in registers; two of doubles are too many
+    extern __shared__ __align__(16) unsigned char scan_shared[];
+    auto& all = *(Shared*)scan_shared;
+    auto& sh = all.f;
+
+    const int tid = threadIdx.x < kThreads ? threadIdx.x : threadIdx.x - kThreads;   // among the walkers, or the helpers
     const int64_t per_group = a.d / a.groups;
     const int64_t per_blocks = blocks / a.groups;
     const int64_t b = blockIdx.x / blocks, blk = blockIdx.x % blocks;
-    const int64_t g = blk / per_blocks, c0 = g * per_group + blk % per_blocks * kChannels, c1 = (g + 1) * per_group;
+    const int64_t g = blk / per_blocks, c0 = g * per_group + blk % per_blocks * kChannels;
+    const int channels = (int)min((g + 1) * per_group - c0, (int64_t)kChannels);
     const int64_t end_all = a.lengths ? min(max((int64_t)a.lengths[b], (int64_t)0), a.t) : a.t;
     const int64_t t0 = blockIdx.y * ck.length;
-    const int64_t stop = min(t0 + ck.length, a.t), end = min(stop, end_all);     // end <= t0: nothing to walk
-    const int64_t bn = (int64_t)a.groups * a.n;
+    const int64_t stop = min(t0 + ck.length, a.t), end = min(stop, end_all);
+    const int64_t steps = max(end - t0, (int64_t)0);
+    const int tiles = (int)((steps + S - 1) / S), last = (int)(steps - (int64_t)(tiles - 1) * S);
+    auto live_of = [&](int tile) { return tile == tiles - 1 ? last : S; };
 
-    // a lane's states and decays
-    const int64_t c = c0 + own;
-    Two<A> h[kPairs], decay[kPairs];
+    // the same for all threads of a warp, which the shuffle lets the compiler know
+    if (__shfl_sync(0xffffffffu, (int)threadIdx.x, 0) < kThreads) {
+        // ---- walkers ----
+        const int lane = tid & (L - 1), own = tid / L;
+        const int64_t c = c0 + own;
+        Two<A> h[kPairs], decay[kPairs];
 #pragma unroll
-    for (int p = 0; p < kPairs; ++p) {
+        for (int p = 0; p < kPairs; ++p) {
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-            const int n = (p * L + lane) * 2 + j;
-            const bool on = n < a.n && c < c1;
-            const int64_t i = c * a.n + n;
-            A v = 0, w = 0;
-            if (on) {
-                w = ((const A*)a.A)[i] * decay_scale<A>();
-                if (!LOCAL && a.state) v = ((const A*)a.state)[b * a.d * a.n + i];
-                if (!LOCAL)
-                    for (int k = 0; k < (int)blockIdx.y; ++k) {
-                        const int64_t q = (b * ck.count + k) * a.d;
-                        const A s = ck.sums[q + c];
-                        v = (s == 0 ? v : power(w * s) * v) + ck.local[q * a.n + i];
-                    }
+            for (int j = 0; j < 2; ++j) {
+                const int n = (p * L + lane) * 2 + j;
+                const bool on = n < a.n && own < channels;
+                const int64_t i = c * a.n + n;
+                A v = 0, w = 0;
+                if (on) {
+                    w = ((const A*)a.A)[i] * decay_scale<A>();
+                    if (!LOCAL && a.state) v = ((const A*)a.state)[b * a.d * a.n + i];
+                    if (!LOCAL)
+                        for (int k = 0; k < (int)blockIdx.y; ++k) {
+                            const int64_t q = (b * ck.count + k) * a.d;
+                            const A s = ck.sums[q + c];
+                            v = (s == 0 ? v : power(w * s) * v) + ck.local[q * a.n + i];
+                        }
+                }
+                (j ? h[p].y : h[p].x) = v;
+                (j ? decay[p].y : decay[p].x) = w;
             }
-            (j ? h[p].y : h[p].x) = v;
-            (j ? decay[p].y : decay[p].x) = w;
         }
+        auto walk = [&](int buf, int live, auto whole) {
+            constexpr bool kWhole = decltype(whole)::value;
+            Two<A> e[kMade][kGroup][kPairs], term[kMade][kGroup][kPairs], cc[kMade][kGroup][kPairs];
+            // a group's exponentials and terms, which wait for no state
+            auto make = [&](int from, int q) {
+#pragma unroll
+                for (int i = 0; i < kGroup; i += 2) {
+                    const Pack<A, 4> u = load_shared<4>(&sh.step[buf][own][from + i][0]);
+#pragma unroll
+                    for (int p = 0; p < kPairs; ++p) {
+                        const Pack<T, 8> w = load_shared<8>(&sh.bc[buf][(from + i) / 2][p][lane][0]);
+#pragma unroll
+                        for (int k = 0; k < 2; ++k) {
+                            const A dt = u.v[2 * k], dtx = u.v[2 * k + 1];
+                            e[q][i + k][p] = {power(dt * decay[p].x), power(dt * decay[p].y)};
+                            term[q][i + k][p] = {dtx * widen(w.v[2 * k]), dtx * widen(w.v[2 * k + 1])};
+                            if (!LOCAL) cc[q][i + k][p] = {widen(w.v[4 + 2 * k]), widen(w.v[5 + 2 * k])};
+                        }
+                    }
+                }
+            };
+            if (kMade == 2) make(0, 0);
+#pragma unroll
+            for (int k = 0; k < kGroups; ++k) {
+                const int from = k * kGroup, q = k & (kMade - 1);
+                if (!kWhole && from >= live) break;
+                if (kMade == 1) make(from, 0);
+                else if (k + 1 < kGroups) make(from + kGroup, q ^ 1);
+#pragma unroll
+                for (int i = 0; i < kGroup; i += 2) {
+                    A sum[2];
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        Two<A> y = {0, 0};
+#pragma unroll
+                        for (int p = 0; p < kPairs; ++p) {
+                            const Two<A> next = fma(e[q][i + j][p], h[p], term[q][i + j][p]);
+                            // behind the end a step is left out: 0 times an infinite A is not 0
+                            if (kWhole || from + i + j < live) h[p] = next;
+                            if (!LOCAL) y = p ? fma(cc[q][i + j][p], h[p], y) : mul(cc[q][i + j][p], h[p]);
+                        }
+                        sum[j] = y.x + y.y;
+                    }
+                    if (!LOCAL) {
+                        // neighbours exchange: even lanes keep the first step, odd ones the second
+                        const bool odd = lane & 1;
+                        const A other = __shfl_xor_sync(0xffffffffu, odd ? sum[0] : sum[1], 1);
+                        sh.y[buf][from + i + odd][own * (L / 2) + lane / 2] = (odd ? sum[1] : sum[0]) + other;
+                    }
+                }
+            }
+        };
+        __syncthreads();
+        for (int i = 0; i < tiles; ++i) {
+            if (live_of(i) == S) walk(i & 1, S, std::true_type());
+            else walk(i & 1, last, std::false_type());
+            __syncthreads();
+        }
+#pragma unroll
+        for (int p = 0; p < kPairs; ++p)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                const int n = (p * L + lane) * 2 + j;
+                if (n >= a.n || own >= channels) continue;
+                const A v = j ? h[p].y : h[p].x;
+                if (LOCAL) ck.local[((b * ck.count + blockIdx.y) * a.d + c) * a.n + n] = v;
+                else if ((int)blockIdx.y == ck.count - 1) ((A*)a.new_state)[(b * a.d + c) * a.n + n] = v;
+            }
+        if (LOCAL) __syncthreads();
+        return;
     }
 
-    // what this thread lays down: x, delta, z of one channel, kRows steps apart, and pieces of B and C
+    // ---- helpers ----
+    // Everything that is the same in every tile is computed here once; in the tiles a helper's time is
+    // its instructions.
     const int row = tid / kChannels, slot = tid % kChannels;
-    const int64_t ch = c0 + slot;
-    const bool mine = ch < c1 && row < kSteps;
-    const A bias = mine && a.delta_bias ? ((const A*)a.delta_bias)[ch] : A(0);
-    const A skip = mine && a.D ? ((const A*)a.D)[ch] : A(0);
-    const int64_t first = (b * a.t + t0 + row) * a.d + ch, stride = kRows * a.d, tile = kSteps * a.d;
-    const T *xs = (const T*)a.x + first, *ds = (const T*)a.delta + first, *zs = a.z ? (const T*)a.z + first : nullptr;
-    T* ys = (T*)a.y + first;
-    const T *bs = (const T*)a.B + (b * a.t + t0) * bn + g * a.n, *cs = (const T*)a.C + (b * a.t + t0) * bn + g * a.n;
+    const bool on = slot < channels;
+    const A bias = on && a.delta_bias ? ((const A*)a.delta_bias)[c0 + slot] : A(0);
+    const A skip = on && a.D ? ((const A*)a.D)[c0 + slot] : A(0);
+    const int64_t bn = (int64_t)a.groups * a.n;
+    const int64_t base = (b * a.t + t0) * a.d + c0, base_b = (b * a.t + t0) * bn + g * a.n;
+    // bytes between the border that a row is copied from and its first value: a tile has an even number
+    // of rows, so they are the same in every tile
+    auto lead = [&](int64_t element) { return piece == 4 ? (int)(element * (int)sizeof(T)) & 3 : 0; };
 
-    T rx[kOwn], rd[kOwn], rz[kOwn], rb[kOwnB], rc[kOwnB];     // requested early, used a tile later
-    A px[kOwn], pz[kOwn];                                     // of the tile being walked: for the skip and the gate
-    A sum = 0;                                                // LOCAL: dt summed over the chunk
+    // what this thread copies: one column of pieces of x, delta, z, B or C, and every `copy_rows`th row
+    const int cols = ((channels * (int)sizeof(T) + (piece == 4 && sizeof(T) == 2 ? 2 : 0)) + piece - 1) / piece;
+    const int cols_b = ((a.n * (int)sizeof(T) + (piece == 4 && sizeof(T) == 2 ? 2 : 0)) + piece - 1) / piece;
+    const int all_cols = 3 * cols + 2 * cols_b;
+    const unsigned ring = (unsigned)__cvta_generic_to_shared(&all.ring[0]);
+    const int copy_rows = max(kHelpers / all_cols, 1), most_cols = (all_cols + kHelpers - 1) / kHelpers;
+    struct Column { const unsigned char* from; unsigned to; int64_t pitch; unsigned row_bytes; };
+    auto column_of = [&](int k) {
+        Column q;
+        const bool bc = k >= 3 * cols;
+        const int which = bc ? 3 + (k - 3 * cols) / cols_b : k / cols, at = (bc ? (k - 3 * cols) % cols_b : k % cols) * piece;
+        const void* array = which == 0 ? a.x : which == 1 ? a.delta : which == 2 ? a.z : which == 3 ? a.B : a.C;
+        q.from = array && k < all_cols && !(LOCAL && (which == 2 || which == 4))
+                     ? (const unsigned char*)array + (bc ? base_b : base) * (int)sizeof(T) + at : nullptr;
+        q.pitch = (bc ? bn : a.d) * (int)sizeof(T);
+        q.row_bytes = bc ? Shared::kRowB : Shared::kRow;
+        q.to = ring + (unsigned)(which < 3 ? which * S * Shared::kRow : 3 * S * Shared::kRow + (which - 3) * S * Shared::kRowB) + at;
+        return q;
+    };
+    const int first_row = most_cols > 1 ? 0 : tid / all_cols;
+    const Column column = column_of(most_cols > 1 ? tid : first_row < copy_rows ? tid % all_cols : all_cols);
+    const unsigned char* column_from = column.from + (column.from ? first_row * column.pitch : 0);
+    int requested = 0;
+    unsigned request_at = 0;                      // stage of the tile requested next, as an offset
+    auto copy_column = [&](const Column& q, const unsigned char* from, int live) {
+        const uintptr_t border = ~(uintptr_t)(piece - 1);
+        const int64_t step = copy_rows * q.pitch;
+        unsigned to = q.to + request_at + first_row * q.row_bytes;
+        for (int r = first_row; r < live; r += copy_rows) {
+            const uintptr_t at = (uintptr_t)from & border;
+            if (piece == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(at) : "memory");
+            else if (sizeof(T) == 8) asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(to), "l"(at) : "memory");
+            else asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(to), "l"(at) : "memory");
+            from += step;
+            to += copy_rows * q.row_bytes;
+        }
+    };
+    auto request = [&]() {
+        if (requested < tiles) {
+            const int live = live_of(requested);
+            if (column.from) {
+                copy_column(column, column_from, live);
+                column_from += S * column.pitch;
+            }
+            for (int m = 1; m < most_cols; ++m) {   // rows of more pieces than there are helpers
+                const Column q = column_of(tid + m * kHelpers);
+                if (q.from) copy_column(q, q.from + (int64_t)requested * S * q.pitch, live);
+            }
+            ++requested;
+            request_at = request_at == (kStages - 1) * sizeof(typename Shared::Stage) ? 0 : request_at + (unsigned)sizeof(typename Shared::Stage);
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");   // one a tile, empty behind the last
+    };
+    // all but the latest kAhead - 2 requests have arrived, for this thread
+    auto arrived = [&]() { asm volatile("cp.async.wait_group %0;" ::"n"(kAhead - 2) : "memory"); };
+
+    // a helper's own values: steps row + i kRows of channel `slot`; and of B and C
+    constexpr int kOwnPairs = (kOwn + 1) / 2;
+    unsigned own_at[kOwn], own_b[kOwnB];          // places in a stage's x, B
+#pragma unroll
+    for (int i = 0; i < kOwn; ++i) {
+        const int s = min(row + i * kRows, S - 1);
+        own_at[i] = (unsigned)(s * Shared::kRow + lead(base + s * a.d) + slot * (int)sizeof(T));
+    }
+#pragma unroll
+    for (int i = 0; i < kOwnB; ++i) {
+        const int e = min(tid + i * kHelpers, S * kStates - 1), s = e / kStates, n = min(e % kStates, a.n - 1);
+        own_b[i] = (unsigned)(3 * S * Shared::kRow + s * Shared::kRowB + lead(base_b + s * bn) + n * (int)sizeof(T));
+    }
+    const unsigned char *lay_at = (const unsigned char*)&all.ring[0], *finish_at = lay_at;
+    const unsigned char* const wrap = lay_at + (kStages - 1) * sizeof(typename Shared::Stage);
+    auto next_stage = [&](const unsigned char*& at) { at = at == wrap ? (const unsigned char*)&all.ring[0] : at + sizeof(typename Shared::Stage); };
     const T zero = narrow<T>(A(0));
-    auto request = [&](int live) {
+    A sum = 0;                                    // LOCAL: dt summed over the chunk
+    auto lay = [&](int buf, int live, auto whole) {
+        constexpr bool kWhole = decltype(whole)::value;
+        Two<A> dt[kOwnPairs], x[kOwnPairs];
+#pragma unroll
+        for (int i = 0; i < kOwnPairs; ++i) {
+            const int k = 2 * i + 1 < kOwn ? 2 * i + 1 : 2 * i;
+            dt[i] = {widen(*(const T*)(lay_at + S * Shared::kRow + own_at[2 * i])), widen(*(const T*)(lay_at + S * Shared::kRow + own_at[k]))};
+            x[i] = {widen(*(const T*)(lay_at + own_at[2 * i])), widen(*(const T*)(lay_at + own_at[k]))};
+            dt[i] = add(dt[i], both(bias));
+        }
+        if (a.softplus) {
+#pragma unroll
+            for (int i = 0; i < kOwnPairs; ++i) dt[i] = softplus(dt[i]);
+        }
 #pragma unroll
         for (int i = 0; i < kOwn; ++i) {
-            const bool on = mine && row + i * kRows < live;
-            rx[i] = on ? xs[i * stride] : zero;
-            rd[i] = on ? ds[i * stride] : zero;
-            if (!LOCAL) rz[i] = on && a.z ? zs[i * stride] : zero;
-        }
-        xs += tile;
-        ds += tile;
-        if (!LOCAL && a.z) zs += tile;
-#pragma unroll
-        for (int i = 0; i < kOwnB; ++i) {
-            const int e = tid + i * kThreads, n = e % kStates, s = e / kStates;
-            const bool on = s < live && n < a.n;
-            rb[i] = on ? bs[s * bn + n] : zero;
-            if (!LOCAL) rc[i] = on ? cs[s * bn + n] : zero;
-        }
-        bs += kSteps * bn;
-        cs += kSteps * bn;
-    };
-    auto lay = [&](int live, int buf) {
-        if (row < kSteps) {
-#pragma unroll
-            for (int i = 0; i < kOwn; ++i) {
-                A dt = widen(rd[i]) + bias;
-                if (a.softplus) dt = softplus(dt);
-                if (!mine || row + i * kRows >= live) dt = 0;
-                const A dtx = dt * widen(rx[i]);
-                sh.step[buf][slot][row + i * kRows] = {{dt, dt}, {dtx, dtx}};
-                if (LOCAL) sum += dt;
-            }
+            const int s = row + i * kRows;
+            A v = i & 1 ? dt[i / 2].y : dt[i / 2].x, w = v * (i & 1 ? x[i / 2].y : x[i / 2].x);
+            if (!kWhole && s >= live) v = w = 0;      // what lies there is left over
+            if (kRows * kOwn > S && s >= S) break;
+            *(Two<A>*)&sh.step[buf][slot][s][0] = {v, w};
+            if (LOCAL) sum += v;
         }
 #pragma unroll
         for (int i = 0; i < kOwnB; ++i) {
-            const int e = tid + i * kThreads;
-            if (kSteps * kStates % kThreads && e >= kSteps * kStates) break;
+            const int e = tid + i * kHelpers;
+            if (S * kStates % kHelpers && e >= S * kStates) break;
             const int s = e / kStates, n = e % kStates;
             const int p = n / (2 * L), l = n % (2 * L) / 2, j = (s & 1) * 2 + (n & 1);
-            ((A*)&sh.b[buf][s / 2][p][l])[j] = widen(rb[i]);
-            if (!LOCAL) ((A*)&sh.c[buf][s / 2][p][l])[j] = widen(rc[i]);
+            T* const to = &sh.bc[buf][s / 2][p][l][j];
+            to[0] = n < a.n ? *(const T*)(lay_at + own_b[i]) : zero;
+            if (!LOCAL) to[4] = n < a.n ? *(const T*)(lay_at + S * Shared::kRowB + own_b[i]) : zero;
         }
+        next_stage(lay_at);
     };
-
-    auto walk = [&](int buf, int live, auto whole) {
+    T* ys = (T*)a.y + base + (int64_t)row * a.d + slot;
+    const int64_t stride = (int64_t)kRows * a.d, tile_stride = (int64_t)S * a.d;
+    auto finish = [&](int buf, int live, auto whole) {
         constexpr bool kWhole = decltype(whole)::value;
+        Two<A> y[kOwnPairs];
 #pragma unroll
-        for (int s0 = 0; s0 < kSteps; s0 += kGroup) {
-            if (!kWhole && s0 >= live) break;
-            Two<A> e[kGroup][kPairs], term[kGroup][kPairs];
-            // all of the group's exponentials and terms, which wait for no state ...
+        for (int i = 0; i < kOwnPairs; ++i) {
+            const int k = 2 * i + 1 < kOwn ? 2 * i + 1 : 2 * i, s0 = min(row + 2 * i * kRows, S - 1), s1 = min(row + k * kRows, S - 1);
+            const Two<A> x = {widen(*(const T*)(finish_at + own_at[2 * i])), widen(*(const T*)(finish_at + own_at[k]))};
+            y[i] = fma(both(skip), x, {lanes_sum<L / 2>(sh.y[buf][s0], slot), lanes_sum<L / 2>(sh.y[buf][s1], slot)});
+        }
+        if (a.z) {
 #pragma unroll
-            for (int i = 0; i < kGroup; i += 2) {
-                const Four<A> u = sh.step[buf][own][s0 + i], v = sh.step[buf][own][s0 + i + 1];
-#pragma unroll
-                for (int p = 0; p < kPairs; ++p) {
-                    const Four<A> bb = sh.b[buf][(s0 + i) / 2][p][lane];
-                    const Two<A> m0 = mul(u.x, decay[p]), m1 = mul(v.x, decay[p]);
-                    e[i][p] = {power(m0.x), power(m0.y)};
-                    e[i + 1][p] = {power(m1.x), power(m1.y)};
-                    term[i][p] = mul(u.y, bb.x);
-                    term[i + 1][p] = mul(v.y, bb.y);
-                }
-            }
-            // ... then the recurrence
-#pragma unroll
-            for (int i = 0; i < kGroup; i += 2) {
-                Two<A> y[2];
-#pragma unroll
-                for (int p = 0; p < kPairs; ++p) {
-                    Four<A> cc;
-                    if (!LOCAL) cc = sh.c[buf][(s0 + i) / 2][p][lane];
-#pragma unroll
-                    for (int k = 0; k < 2; ++k) {
-                        const Two<A> next = fma(e[i + k][p], h[p], term[i + k][p]);
-                        // behind the end a step is left out: 0 times an infinite A is not 0
-                        if (kWhole || s0 + i + k < live) h[p] = next;
-                        if (!LOCAL) y[k] = p ? fma(k ? cc.y : cc.x, h[p], y[k]) : mul(k ? cc.y : cc.x, h[p]);
-                    }
-                }
-                if (!LOCAL) {
-                    sh.y[buf][s0 + i][tid] = y[0].x + y[0].y;
-                    sh.y[buf][s0 + i + 1][tid] = y[1].x + y[1].y;
-                }
+            for (int i = 0; i < kOwnPairs; ++i) {
+                const int k = 2 * i + 1 < kOwn ? 2 * i + 1 : 2 * i;
+                const unsigned char* const z = finish_at + 2 * S * Shared::kRow;
+                y[i] = mul(y[i], gate(Two<A>{widen(*(const T*)(z + own_at[2 * i])), widen(*(const T*)(z + own_at[k]))}));
             }
         }
-    };
-
-    auto keep = [&]() {
 #pragma unroll
-        for (int i = 0; i < kOwn; ++i) {
-            px[i] = widen(rx[i]);
-            if (!LOCAL) pz[i] = widen(rz[i]);
-        }
+        for (int i = 0; i < kOwn; ++i)
+            if (on && (kRows * kOwn == S && kWhole ? true : row + i * kRows < live)) ys[i * stride] = narrow<T>(i & 1 ? y[i / 2].y : y[i / 2].x);
+        ys += tile_stride;
+        next_stage(finish_at);
     };
-
-    if (t0 < end) {
-        int live = (int)min(end - t0, (int64_t)kSteps);
-        request(live);
-        lay(live, 0);
-        keep();
+    auto lay_tile = [&](int tile) {
+        if (tile < tiles - 1 || last == S) lay(tile & 1, S, std::true_type());
+        else lay(tile & 1, last, std::false_type());
+    };
+    auto finish_tile = [&](int tile) {
+        if (tile < tiles - 1 || last == S) finish(tile & 1, S, std::true_type());
+        else finish(tile & 1, last, std::false_type());
+    };
+    for (int i = 0; i < kAhead; ++i) request();
+    arrived();
+    asm volatile("bar.sync 1, %0;" ::"n"(kHelpers) : "memory");     // tiles 0 and 1 are there for every helper
+    if (tiles > 0) lay_tile(0);
+    __syncthreads();
+    for (int i = 0; i < tiles; ++i) {
+        // tile i is walked: request i + kAhead, into the place of i - 2; finish i - 1, lay i + 1
+        request();
+        if (!LOCAL && i > 0) finish_tile(i - 1);
+        if (i + 1 < tiles) lay_tile(i + 1);
+        arrived();           // tile i + 2, which the next turn lays down
         __syncthreads();
-        int buf = 0;
-        for (int64_t t = t0; t < end; t += kSteps, buf ^= 1) {
-            const int next = (int)min(max(end - t - kSteps, (int64_t)0), (int64_t)kSteps);
-            if (next) request(next);
-            if (live == kSteps) walk(buf, live, std::true_type());
-            else walk(buf, live, std::false_type());
-            if (next) lay(next, buf ^ 1);
-            __syncthreads();
-            if (!LOCAL) {
-#pragma unroll
-                for (int i = 0; i < kOwn; ++i) {
-                    if (!mine || row + i * kRows >= live) continue;
-                    A y = lanes_sum<L>(sh.y[buf][row + i * kRows], slot) + skip * px[i];
-                    if (a.z) y *= gate(pz[i]);
-                    ys[i * stride] = narrow<T>(y);
-                }
-                ys += tile;
-            }
-            if (next) keep();
-            live = next;
-        }
     }
     if (LOCAL) {
-        // dt of a channel was summed by kRows threads: add them up in their order
-        __syncthreads();
+        // dt of a channel was summed by up to kRows helpers: add them up in their order
         A* const part = (A*)&sh.step;
-        part[tid] = sum;
+        part[tid] = row < S ? sum : A(0);
         __syncthreads();
-        if (tid < kChannels && c0 + tid < c1) {
+        if (tid < channels) {
             A s = 0;
-            for (int i = tid; i < kThreads; i += kChannels) s += part[i];
+            for (int i = tid; i < kHelpers; i += kChannels) s += part[i];
             ck.sums[(b * ck.count + blockIdx.y) * a.d + c0 + tid] = s;
         }
-    } else {
-        // rows behind the end of the sequence
-        const int64_t from = max(end, t0);
-        for (int64_t e = tid; e < (stop - from) * kChannels; e += kThreads) {
-            const int64_t cc = c0 + e % kChannels;
-            if (cc < c1) ((T*)a.y)[(b * a.t + from + e / kChannels) * a.d + cc] = zero;
-        }
-        if ((int)blockIdx.y != ck.count - 1) return;
+        return;
     }
-#pragma unroll
-    for (int p = 0; p < kPairs; ++p)
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-            const int n = (p * L + lane) * 2 + j;
-            if (n >= a.n || c >= c1) continue;
-            const A v = j ? h[p].y : h[p].x;
-            if (LOCAL) ck.local[((b * ck.count + blockIdx.y) * a.d + c) * a.n + n] = v;
-            else ((A*)a.new_state)[(b * a.d + c) * a.n + n] = v;
-        }
+    if (tiles > 0) finish_tile(tiles - 1);
+    // rows behind the end of the sequence
+    const int64_t behind = max(end, t0);
+    for (int64_t e = tid; e < (stop - behind) * kChannels; e += kHelpers) {
+        const int cc = (int)(e % kChannels);
+        if (cc < channels) ((T*)a.y)[(b * a.t + behind + e / kChannels) * a.d + c0 + cc] = zero;
+    }
 }
 
 // ---- single tokens ------------------------------------------------------------------------------------
@@ -434,41 +573,48 @@ cudaError_t token(const SelectiveScanArgs& a, cudaStream_t s) {
 
 // ---- launches -------------------------------------------------------------------------------------------
 
-int lanes_for(int n) { return n <= 4 ? 2 : n <= 8 ? 4 : n <= 64 ? 8 : n <= 128 ? 16 : 32; }
+int lanes_for(int n) { return n <= 8 ? 4 : n <= 64 ? 8 : n <= 128 ? 16 : 32; }
 
 int64_t channel_blocks(const SelectiveScanArgs& a) {
     const int64_t channels = kThreads / lanes_for(a.n);
     return a.groups * ((a.d / a.groups + channels - 1) / channels);
 }
 
+constexpr int kBorder = 32;     // chunks begin at multiples of every tile's steps
+
 // Chunks of the time axis: none while the channels' blocks give half of the SMs one each, since
 // chunks compute every exponential twice; else as many as make two blocks an SM, of at least 64 steps.
 template <typename A>
 ScanChunks<A> chunks_for(const SelectiveScanArgs& a, int sm_count) {
     ScanChunks<A> ck;
-    ck.length = std::max<int64_t>((a.t + kSteps - 1) / kSteps, 1) * kSteps;
+    ck.length = std::max<int64_t>((a.t + kBorder - 1) / kBorder, 1) * kBorder;
     const int64_t blocks = channel_blocks(a) * a.b;
     if (2 * blocks >= sm_count || a.t < 128) return ck;
     const int64_t want = std::min<int64_t>(2 * sm_count / blocks, a.t / 64);
-    ck.length = ((a.t + want - 1) / want + kSteps - 1) / kSteps * kSteps;
+    ck.length = ((a.t + want - 1) / want + kBorder - 1) / kBorder * kBorder;
     ck.count = (int)((a.t + ck.length - 1) / ck.length);
     return ck;
 }
 
-template <typename T, int L, int N, bool LOCAL>
-cudaError_t scan_pass(const SelectiveScanArgs& a, const ScanChunks<typename Acc<T>::type>& ck, int64_t blocks, int count, cudaStream_t s) {
-    constexpr size_t bytes = sizeof(ScanShared<typename Acc<T>::type, L, N, LOCAL>);
+template <typename T, int L, int N, int S, bool LOCAL>
+cudaError_t scan_pass(const SelectiveScanArgs& a, const ScanChunks<typename Acc<T>::type>& ck, int64_t blocks, int count, int piece, cudaStream_t s) {
+    constexpr size_t bytes = sizeof(ScanShared<T, L, N, S, LOCAL>);
+    const auto kernel = scan_kernel<T, L, N, S, LOCAL>;
     if (bytes > 48 * 1024) {
-        const cudaError_t e = cudaFuncSetAttribute(scan_kernel<T, L, N, LOCAL>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
         if (e != cudaSuccess) return e;
     }
-    scan_kernel<T, L, N, LOCAL><<<dim3((unsigned)(blocks * a.b), count), kThreads, bytes, s>>>(a, ck, (int)blocks);
+    kernel<<<dim3((unsigned)(blocks * a.b), count), kThreads + kHelpers, bytes, s>>>(a, ck, (int)blocks, piece);
     return cudaGetLastError();
 }
 
 template <typename T, int L, int N>
 cudaError_t prompt(const SelectiveScanArgs& a, int sm_count, cudaStream_t s) {
     using A = typename Acc<T>::type;
+    // tiles as long as shared memory allows, twice where two blocks can share an SM
+    constexpr int S = sizeof(T) == 2 && N == 2 ? 32 : sizeof(T) == 8 && L > 8 ? 8 : 16;
+    const int64_t rows = a.d / a.groups * (int64_t)sizeof(T), rows_b = a.n * (int64_t)sizeof(T);
+    const int piece = rows % 16 == 0 && rows_b % 16 == 0 ? 16 : sizeof(T) == 8 ? 8 : 4;
     ScanChunks<A> ck = chunks_for<A>(a, sm_count);
     const int64_t blocks = channel_blocks(a);
     if (blocks * a.b >= (1LL << 31)) return cudaErrorInvalidValue;
@@ -476,16 +622,15 @@ cudaError_t prompt(const SelectiveScanArgs& a, int sm_count, cudaStream_t s) {
         ck.local = (A*)a.workspace;
         ck.sums = ck.local + a.b * ck.count * a.d * a.n;
         // the last chunk's states are never entered from
-        const cudaError_t e = scan_pass<T, L, N, true>(a, ck, blocks, ck.count - 1, s);
+        const cudaError_t e = scan_pass<T, L, N, S, true>(a, ck, blocks, ck.count - 1, piece, s);
         if (e != cudaSuccess) return e;
     }
-    return scan_pass<T, L, N, false>(a, ck, blocks, ck.count, s);
+    return scan_pass<T, L, N, S, false>(a, ck, blocks, ck.count, piece, s);
 }
 
 template <typename T>
 cudaError_t scan(const SelectiveScanArgs& a, int sm_count, cudaStream_t s) {
     if (a.t == 1) return token<T>(a, s);
-    if (a.n <= 4) return prompt<T, 2, 2>(a, sm_count, s);
     if (a.n <= 8) return prompt<T, 4, 2>(a, sm_count, s);
     if (a.n <= 16) return prompt<T, 8, 2>(a, sm_count, s);
     if (a.n <= 32) return prompt<T, 8, 4>(a, sm_count, s);
