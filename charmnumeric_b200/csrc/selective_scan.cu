@@ -141,7 +141,10 @@ struct ScanShared {
     static constexpr int kRow = kChannels * (int)sizeof(T) + 16, kRowB = kStates * (int)sizeof(T) + 16;
     struct Fixed {
         alignas(16) A step[2][kChannels][S + 2][2];            // dt, dt x
-        alignas(16) T bc[2][S / 2][kPairs][L][8];              // a lane's pairs of B of two steps, and of C
+        // a lane's pairs of B of two steps and of C, eight values, in pieces of 16 bytes that lie side by
+        // side for the lanes
+        static constexpr int kPiece = 16 / (int)sizeof(T);
+        alignas(16) T bc[2][S / 2][kPairs][8 / kPiece][L][kPiece];
         alignas(16) A y[2][S][kPitch];                         // L / 2 sums of each channel
     };
     struct alignas(16) Stage {
@@ -175,13 +178,13 @@ __device__ __forceinline__ A lanes_sum(const A* y, int slot) {
     return t;
 }
 
+// V values in accesses of 16 bytes, `apart` values from one to the next
 template <int V, typename A>
-__device__ __forceinline__ Pack<A, V> load_shared(const A* p) {
-    // 16 bytes an access
+__device__ __forceinline__ Pack<A, V> load_shared(const A* p, int apart) {
     constexpr int W = 16 / (int)sizeof(A);
     Pack<A, V> r;
 #pragma unroll
-    for (int i = 0; i < V; i += W) *(Pack<A, W>*)&r.v[i] = *(const Pack<A, W>*)(p + i);
+    for (int i = 0; i < V / W; ++i) *(Pack<A, W>*)&r.v[i * W] = *(const Pack<A, W>*)(p + i * apart);
     return r;
 }
 
@@ -252,10 +255,10 @@ __global__ void __launch_bounds__(kThreads + kHelpers, sizeof(T) <= 4 && N == 2 
             auto make = [&](int from, int q) {
 #pragma unroll
                 for (int i = 0; i < kGroup; i += 2) {
-                    const Pack<A, 4> u = load_shared<4>(&sh.step[buf][own][from + i][0]);
+                    const Pack<A, 4> u = load_shared<4>(&sh.step[buf][own][from + i][0], 16 / (int)sizeof(A));
 #pragma unroll
                     for (int p = 0; p < kPairs; ++p) {
-                        const Pack<T, 8> w = load_shared<8>(&sh.bc[buf][(from + i) / 2][p][lane][0]);
+                        const Pack<T, 8> w = load_shared<8>(&sh.bc[buf][(from + i) / 2][p][0][lane][0], 16 * L / (int)sizeof(T));
 #pragma unroll
                         for (int k = 0; k < 2; ++k) {
                             const A dt = u.v[2 * k], dtx = u.v[2 * k + 1];
@@ -433,9 +436,9 @@ __global__ void __launch_bounds__(kThreads + kHelpers, sizeof(T) <= 4 && N == 2 
             if (S * kStates % kHelpers && e >= S * kStates) break;
             const int s = e / kStates, n = e % kStates;
             const int p = n / (2 * L), l = n % (2 * L) / 2, j = (s & 1) * 2 + (n & 1);
-            T* const to = &sh.bc[buf][s / 2][p][l][j];
-            to[0] = n < a.n ? *(const T*)(lay_at + own_b[i]) : zero;
-            if (!LOCAL) to[4] = n < a.n ? *(const T*)(lay_at + S * Shared::kRowB + own_b[i]) : zero;
+            constexpr int W = 16 / (int)sizeof(T);
+            sh.bc[buf][s / 2][p][j / W][l][j % W] = n < a.n ? *(const T*)(lay_at + own_b[i]) : zero;
+            if (!LOCAL) sh.bc[buf][s / 2][p][(4 + j) / W][l][(4 + j) % W] = n < a.n ? *(const T*)(lay_at + S * Shared::kRowB + own_b[i]) : zero;
         }
         next_stage(lay_at);
     };
