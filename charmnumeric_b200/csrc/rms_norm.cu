@@ -20,8 +20,197 @@ using namespace seq;
 
 namespace {
 
+// A row is read once and stays in registers: W warps have a row, a thread R pieces of V neighbouring
+// values (16 bytes), W * 32 pieces apart.  Bound by HBM.  One warp a row for short rows (no barrier;
+// four rows a block), up to 32 for long ones; rows longer than that are read twice, the second time
+// from L2.  Pieces begin at 16-byte borders of the arrays, which all have the same ones: where n is no
+// multiple of V a row's first and last piece are partly its neighbours' (WHOLE = false) and are moved
+// value by value.
+template <typename T, int V, int R, int W, bool RESIDUAL, bool WHOLE>
+struct Row {
+    using A = typename Acc<T>::type;
+    int64_t base;            // of the row in its array
+    int n, first;            // column of this thread's first value; before column 0 for some first pieces
+    Pack<T, V> x[R], r[RESIDUAL ? R : 1];
+
+    __device__ __forceinline__ int at(int i) const { return first + i * (W * 32 * V); }
+    __device__ __forceinline__ bool any(int i) const { return at(i) < n; }
+    __device__ __forceinline__ bool all(int i) const { return WHOLE || (at(i) >= 0 && at(i) + V <= n); }
+    __device__ __forceinline__ bool has(int i, int j) const { return WHOLE || (at(i) + j >= 0 && at(i) + j < n); }
+
+    // piece i of an array of rows; what is not the row's is left as it is
+    template <typename U>
+    __device__ __forceinline__ void get(Pack<U, V>& to, const U* from, int i) const {
+        if (all(i)) {
+            to = *(const Pack<U, V>*)(from + base + at(i));
+        } else {
+#pragma unroll
+            for (int j = 0; j < V; ++j)
+                if (has(i, j)) to.v[j] = from[base + at(i) + j];
+        }
+    }
+    template <typename U>
+    __device__ __forceinline__ void put(const Pack<U, V>& from, U* to, int i) const {
+        if (all(i)) {
+            *(Pack<U, V>*)(to + base + at(i)) = from;
+        } else {
+#pragma unroll
+            for (int j = 0; j < V; ++j)
+                if (has(i, j)) to[base + at(i) + j] = from.v[j];
+        }
+    }
+    __device__ __forceinline__ void load(const RmsNormArgs& a, int64_t row, int tid) {
+        base = row * a.n;
+        n = (int)a.n;
+        first = tid * V - (WHOLE ? 0 : (int)(base % V));
+#pragma unroll
+        for (int i = 0; i < R; ++i) {
+            if (!any(i)) break;
+            get(x[i], (const T*)a.x, i);
+            if (RESIDUAL) get(r[i], (const T*)a.residual, i);
+        }
+    }
+    // columns of the weight, which begin at other borders than a row's
+    __device__ __forceinline__ void weight(A (&w)[V], const RmsNormArgs& a, int i) const {
+        if (WHOLE && a.weight) {
+            const Pack<T, V> v = *(const Pack<T, V>*)((const T*)a.weight + at(i));
+#pragma unroll
+            for (int j = 0; j < V; ++j) w[j] = widen(v.v[j]);
+        } else {
+#pragma unroll
+            for (int j = 0; j < V; ++j) w[j] = a.weight && has(i, j) ? widen(((const T*)a.weight)[at(i) + j]) : A(1);
+        }
+    }
+    __device__ __forceinline__ A sum(int i, int j) const {
+        const A v = widen(x[i].v[j]);
+        return RESIDUAL ? v + widen(r[i].v[j]) : v;
+    }
+};
+
+template <typename A>
+__device__ __forceinline__ A root(A squares, const RmsNormArgs& a) {
+    return A(1) / sqrt(squares / (A)a.n + (A)a.eps);
+}
+
+template <typename T, int V, int R, int W, bool RESIDUAL, bool WHOLE>
+__global__ void __launch_bounds__(W == 1 ? 128 : W * 32) rms_norm_kernel(RmsNormArgs a) {
+    using A = typename Acc<T>::type;
+    const int64_t row = W == 1 ? (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5) : blockIdx.x;
+    if (row >= a.rows) return;
+    Row<T, V, R, W, RESIDUAL, WHOLE> in;
+    in.load(a, row, W == 1 ? threadIdx.x & 31 : threadIdx.x);
+    A s = 0;
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+        if (!in.any(i)) break;
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            const A h = in.sum(i, j);
+            if (in.has(i, j)) s += h * h;
+        }
+    }
+    if (W == 1) {
+        s = warp_sum(s);
+    } else {
+        __shared__ A sm[W];
+        s = block_sum(s, sm);
+    }
+    const A r = root(s, a);
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+        if (!in.any(i)) break;
+        Pack<T, V> y, h;
+        A w[V];
+        in.weight(w, a, i);
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            const A v = in.sum(i, j);
+            h.v[j] = narrow<T>(v);
+            y.v[j] = narrow<T>(v * r * w[j]);
+        }
+        in.put(y, (T*)a.y, i);
+        if (RESIDUAL) in.put(h, (T*)a.h, i);
+    }
+}
+
+// The same with the 8-bit output.  The lanes that share a group of columns find its largest value
+// together: G lanes for groups of G pieces (a power of two up to a warp), or the whole block for one
+// scale a row (G = 0).
+template <typename T, int V, int R, int W, int G, bool RESIDUAL, bool WHOLE>
+__global__ void __launch_bounds__(W == 1 ? 128 : W * 32) rms_norm_8_kernel(RmsNormArgs a) {
+    using A = typename Acc<T>::type;
+    const int tid = W == 1 ? threadIdx.x & 31 : threadIdx.x;
+    const int64_t row = W == 1 ? (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5) : blockIdx.x;
+    if (row >= a.rows) return;
+    Row<T, V, R, W, RESIDUAL, WHOLE> in;
+    in.load(a, row, tid);
+    A s = 0, most[R];
+    // a NaN counts as infinity: it makes the group's scale NaN like one
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+        most[i] = 0;
+        if (in.any(i)) {
+            A w[V];
+            in.weight(w, a, i);
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                const A h = in.sum(i, j), v = fabs(h * w[j]);
+                if (!in.has(i, j)) continue;
+                s += h * h;
+                most[i] = v <= most[i] ? most[i] : v == v ? v : (A)INFINITY;
+            }
+        }
+    }
+    __shared__ A sm[W], sm_most[W];
+    if (G == 0) {
+#pragma unroll
+        for (int i = 1; i < R; ++i) most[0] = most[i] > most[0] ? most[i] : most[0];
+        most[0] = warp_max(most[0]);
+        if (W > 1 && (tid & 31) == 0) sm_most[tid >> 5] = most[0];
+    } else {
+#pragma unroll
+        for (int i = 0; i < R; ++i)
+#pragma unroll
+            for (int o = G / 2; o > 0; o >>= 1) {
+                const A v = __shfl_xor_sync(0xffffffffu, most[i], o);
+                most[i] = v > most[i] ? v : most[i];
+            }
+    }
+    s = W == 1 ? warp_sum(s) : block_sum(s, sm);    // its barrier covers sm_most
+    if (G == 0) {
+        if (W > 1)
+#pragma unroll
+            for (int i = 0; i < W; ++i) most[0] = sm_most[i] > most[0] ? sm_most[i] : most[0];
+#pragma unroll
+        for (int i = 1; i < R; ++i) most[i] = most[0];
+    }
+    const A r = root(s, a);
+    const int64_t groups = (a.n + a.group - 1) / a.group;
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+        if (!in.any(i)) break;
+        const bool fine = most[i] < (A)INFINITY;
+        const A f = fine && most[i] > 0 ? A(127) / most[i] : A(0);
+        Pack<T, V> h;
+        Pack<signed char, V> q;
+        A w[V];
+        in.weight(w, a, i);
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            const A v = in.sum(i, j);
+            h.v[j] = narrow<T>(v);
+            q.v[j] = fine ? (signed char)(int)rint(v * w[j] * f) : (signed char)0;
+        }
+        in.put(q, (signed char*)a.y, i);
+        if (RESIDUAL) in.put(h, (T*)a.h, i);
+        if (G == 0 ? tid == 0 && i == 0 : tid % (G ? G : 1) == 0)
+            ((A*)a.scale)[row * groups + (G == 0 ? 0 : in.at(i) / (int)a.group)] = fine ? most[i] * r / A(127) : (A)NAN;
+    }
+}
+
+// Any length, any group, any alignment; a block a row, which is read again for the results.
 template <typename T>
-__global__ void __launch_bounds__(256) rms_norm_kernel(RmsNormArgs a) {
+__global__ void __launch_bounds__(256) rms_norm_long_kernel(RmsNormArgs a) {
     using A = typename Acc<T>::type;
     __shared__ A sm[8];
     const int64_t row = blockIdx.x;
@@ -35,7 +224,7 @@ __global__ void __launch_bounds__(256) rms_norm_kernel(RmsNormArgs a) {
         s += h * h;
     }
     s = block_sum(s, sm);
-    const A r = A(1) / sqrt(s / (A)a.n + (A)a.eps);
+    const A r = root(s, a);
     if (a.group == 0) {
         for (int64_t i = threadIdx.x; i < a.n; i += 256) {
             A h = widen(x[i]);
@@ -52,7 +241,6 @@ __global__ void __launch_bounds__(256) rms_norm_kernel(RmsNormArgs a) {
     for (int64_t g = threadIdx.x >> 5; g < groups; g += 8) {
         const int64_t i0 = g * a.group, i1 = min(i0 + a.group, a.n);
         A most = 0;
-        bool nan = false;
         for (int64_t i = i0 + lane; i < i1; i += 32) {
             A h = widen(x[i]);
             if (res) {
@@ -60,20 +248,83 @@ __global__ void __launch_bounds__(256) rms_norm_kernel(RmsNormArgs a) {
                 ((T*)a.h)[row * a.n + i] = narrow<T>(h);
             }
             const A v = fabs(w ? h * widen(w[i]) : h);
-            nan |= v != v;
-            most = v > most ? v : most;
+            most = v <= most ? most : v == v ? v : (A)INFINITY;
         }
         most = warp_max(most);
-        const bool bad = __any_sync(0xffffffffu, nan) || isinf(most);
-        const A f = most > 0 && !bad ? A(127) / most : A(0);
+        const bool fine = most < (A)INFINITY;
+        const A f = most > 0 && fine ? A(127) / most : A(0);
         for (int64_t i = i0 + lane; i < i1; i += 32) {
             A h = widen(x[i]);
             if (res) h += widen(res[i]);
             const A v = w ? h * widen(w[i]) : h;
-            ((signed char*)a.y)[row * a.n + i] = bad ? 0 : (signed char)(int)rint(v * f);
+            ((signed char*)a.y)[row * a.n + i] = fine ? (signed char)(int)rint(v * f) : (signed char)0;
         }
-        if (lane == 0) ((A*)a.scale)[row * groups + g] = bad ? (A)NAN : most * r / A(127);
+        if (lane == 0) ((A*)a.scale)[row * groups + g] = fine ? most * r / A(127) : (A)NAN;
     }
+}
+
+// ---- variants ---------------------------------------------------------------------------------------------
+
+template <typename T, int V, int R, int W, bool WHOLE>
+cudaError_t launch_row(const RmsNormArgs& a, cudaStream_t s) {
+    const unsigned blocks = (unsigned)(W == 1 ? (a.rows + 3) / 4 : a.rows), threads = W == 1 ? 128 : W * 32;
+    if (a.residual) rms_norm_kernel<T, V, R, W, true, WHOLE><<<blocks, threads, 0, s>>>(a);
+    else rms_norm_kernel<T, V, R, W, false, WHOLE><<<blocks, threads, 0, s>>>(a);
+    return cudaGetLastError();
+}
+
+template <typename T, int V, int R, int W, int G, bool WHOLE>
+cudaError_t launch_row_8(const RmsNormArgs& a, cudaStream_t s) {
+    const unsigned blocks = (unsigned)(W == 1 ? (a.rows + 3) / 4 : a.rows), threads = W == 1 ? 128 : W * 32;
+    if (a.residual) rms_norm_8_kernel<T, V, R, W, G, true, WHOLE><<<blocks, threads, 0, s>>>(a);
+    else rms_norm_8_kernel<T, V, R, W, G, false, WHOLE><<<blocks, threads, 0, s>>>(a);
+    return cudaGetLastError();
+}
+
+template <typename T>
+cudaError_t launch_long(const RmsNormArgs& a, cudaStream_t s) {
+    rms_norm_long_kernel<T><<<(unsigned)a.rows, 256, 0, s>>>(a);
+    return cudaGetLastError();
+}
+
+// One warp for up to 4 pieces a thread, else as few warps as hold the row in 4 pieces a thread.
+template <typename T, bool WHOLE>
+cudaError_t by_length(const RmsNormArgs& a, cudaStream_t s) {
+    constexpr int V = 16 / sizeof(T);
+    const int64_t pieces = (a.n + V - 1) / V + !WHOLE;
+    if (pieces <= 32) return launch_row<T, V, 1, 1, WHOLE>(a, s);
+    if (pieces <= 128) return launch_row<T, V, 4, 1, WHOLE>(a, s);
+    if (pieces <= 256) return launch_row<T, V, 2, 4, WHOLE>(a, s);
+    if (pieces <= 512) return launch_row<T, V, 4, 4, WHOLE>(a, s);
+    if (pieces <= 1024) return launch_row<T, V, 4, 8, WHOLE>(a, s);
+    if (pieces <= 2048) return launch_row<T, V, 4, 16, WHOLE>(a, s);
+    if (pieces <= 4096) return launch_row<T, V, 4, 32, WHOLE>(a, s);
+    return launch_long<T>(a, s);
+}
+
+template <typename T, int G, bool WHOLE>
+cudaError_t by_length_8(const RmsNormArgs& a, cudaStream_t s) {
+    constexpr int V = 16 / sizeof(T);
+    const int64_t pieces = (a.n + V - 1) / V + !WHOLE;
+    if (pieces <= 128) return launch_row_8<T, V, 4, 1, G, WHOLE>(a, s);
+    if (pieces <= 512) return launch_row_8<T, V, 4, 4, G, WHOLE>(a, s);
+    if (pieces <= 1024) return launch_row_8<T, V, 4, 8, G, WHOLE>(a, s);
+    if (pieces <= 2048) return launch_row_8<T, V, 4, 16, G, WHOLE>(a, s);
+    return launch_long<T>(a, s);
+}
+
+template <typename T>
+cudaError_t rms_norm(const RmsNormArgs& a, cudaStream_t s) {
+    constexpr int V = 16 / sizeof(T);
+    const bool whole = a.n % V == 0;
+    if (a.group == 0) return whole ? by_length<T, true>(a, s) : by_length<T, false>(a, s);
+    if (a.group >= a.n) return whole ? by_length_8<T, 0, true>(a, s) : by_length_8<T, 0, false>(a, s);
+    // groups of a power of two of pieces are shared by neighbouring lanes
+    if (whole && a.group == 4 * V) return by_length_8<T, 4, true>(a, s);
+    if (whole && a.group == 8 * V) return by_length_8<T, 8, true>(a, s);
+    if (whole && a.group == 16 * V) return by_length_8<T, 16, true>(a, s);
+    if (whole && a.group == 32 * V) return by_length_8<T, 32, true>(a, s);
+    return launch_long<T>(a, s);
 }
 
 // ---- conversions ------------------------------------------------------------------------------------
@@ -132,14 +383,12 @@ cudaError_t dequantize_to(const ConvertArgs& a, int grid, cudaStream_t s) {
 cudaError_t launch_rms_norm(const RmsNormArgs& a, int sm_count, cudaStream_t s) {
     (void)sm_count;
     if (a.rows >= (1LL << 31)) return cudaErrorInvalidValue;
-    const int grid = (int)a.rows;
     switch (a.dtype) {
-        case DT_F16: rms_norm_kernel<__half><<<grid, 256, 0, s>>>(a); break;
-        case DT_F32: rms_norm_kernel<float><<<grid, 256, 0, s>>>(a); break;
-        case DT_F64: rms_norm_kernel<double><<<grid, 256, 0, s>>>(a); break;
+        case DT_F16: return rms_norm<__half>(a, s);
+        case DT_F32: return rms_norm<float>(a, s);
+        case DT_F64: return rms_norm<double>(a, s);
         default: return cudaErrorInvalidValue;
     }
-    return cudaGetLastError();
 }
 
 cudaError_t launch_convert(const ConvertArgs& a, int sm_count, cudaStream_t s) {

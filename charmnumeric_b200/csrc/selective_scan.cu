@@ -511,67 +511,94 @@ __global__ void __launch_bounds__(kThreads + kHelpers, sizeof(T) <= 4 && N == 2 
 
 // ---- single tokens ------------------------------------------------------------------------------------
 //
-// The states are read and written once: a lane has V neighbouring states (16 bytes where n allows),
-// `lanes` lanes a channel.  An inactive sequence's states are copied.
-template <typename T, int V>
+// The states are read and written once: a lane has V neighbouring states of a channel (16 bytes where n
+// allows), `lanes` lanes the channel, and M sequences at a time, whose loads are all on their way
+// before the first is used.  An inactive sequence's states are copied.
+template <typename T, int V, int M>
 __global__ void __launch_bounds__(kThreads) scan_token_kernel(SelectiveScanArgs a, int lanes) {
     using A = typename Acc<T>::type;
-    const int64_t at = ((int64_t)blockIdx.x * kThreads + threadIdx.x) / lanes;   // b d + c
     const int lane = threadIdx.x & (lanes - 1);
-    const bool on = at < a.b * a.d;
-    const int64_t b = on ? at / a.d : 0, c = on ? at - b * a.d : 0;
-    const bool live = on && !(a.lengths && a.lengths[b] < 1);
-    const int64_t bn = (int64_t)a.groups * a.n;
-    const T* const bs = (const T*)a.B + b * bn + c / (a.d / a.groups) * a.n;
-    const T* const cs = (const T*)a.C + b * bn + c / (a.d / a.groups) * a.n;
-    A x = 0, dt = 0, y = 0;
-    if (live) {
-        x = widen(((const T*)a.x)[at]);
-        dt = widen(((const T*)a.delta)[at]) + (a.delta_bias ? ((const A*)a.delta_bias)[c] : A(0));
-        if (a.softplus) dt = softplus(dt);
-    }
-    const A dtx = dt * x;
-    if (on) {
+    const int64_t c = ((int64_t)blockIdx.x * kThreads + threadIdx.x) / lanes;
+    const bool on = c < a.d;
+    const int64_t bn = (int64_t)a.groups * a.n, g = on ? c / (a.d / a.groups) * a.n : 0;
+    const A bias = on && a.delta_bias ? ((const A*)a.delta_bias)[c] : A(0), skip = on && a.D ? ((const A*)a.D)[c] : A(0);
+    for (int64_t b0 = (int64_t)blockIdx.y * M; b0 < a.b; b0 += (int64_t)gridDim.y * M) {
+        A x[M], dt[M], z[M], y[M];
+        bool here[M], live[M];
+#pragma unroll
+        for (int k = 0; k < M; ++k) {
+            const int64_t b = b0 + k;
+            here[k] = on && b < a.b;
+            live[k] = here[k] && !(a.lengths && a.lengths[b] < 1);
+            x[k] = live[k] ? widen(((const T*)a.x)[b * a.d + c]) : A(0);
+            dt[k] = live[k] ? widen(((const T*)a.delta)[b * a.d + c]) : A(0);
+            z[k] = live[k] && a.z ? widen(((const T*)a.z)[b * a.d + c]) : A(0);
+            y[k] = 0;
+        }
         for (int n = lane * V; n < a.n; n += lanes * V) {
-            Pack<A, V> h, w;
-            if (a.state) h = *(const Pack<A, V>*)((const A*)a.state + at * a.n + n);
-            else
+            Pack<A, V> h[M], w;
+            Pack<T, V> bb[M], cc[M];
 #pragma unroll
-                for (int j = 0; j < V; ++j) h.v[j] = 0;
-            if (live) {
-                w = *(const Pack<A, V>*)((const A*)a.A + c * a.n + n);
-                const Pack<T, V> bb = *(const Pack<T, V>*)(bs + n), cc = *(const Pack<T, V>*)(cs + n);
+            for (int j = 0; j < V; ++j) w.v[j] = on ? ((const A*)a.A)[c * a.n + n + j] * decay_scale<A>() : A(0);
 #pragma unroll
-                for (int j = 0; j < V; ++j) {
-                    h.v[j] = power(dt * (w.v[j] * decay_scale<A>())) * h.v[j] + dtx * widen(bb.v[j]);
-                    y += widen(cc.v[j]) * h.v[j];
+            for (int k = 0; k < M; ++k) {
+                const int64_t b = b0 + k;
+#pragma unroll
+                for (int j = 0; j < V; ++j) h[k].v[j] = 0;
+                if (here[k] && a.state) h[k] = *(const Pack<A, V>*)((const A*)a.state + (b * a.d + c) * a.n + n);
+                if (live[k]) {
+                    bb[k] = *(const Pack<T, V>*)((const T*)a.B + b * bn + g + n);
+                    cc[k] = *(const Pack<T, V>*)((const T*)a.C + b * bn + g + n);
                 }
             }
-            *(Pack<A, V>*)((A*)a.new_state + at * a.n + n) = h;
+#pragma unroll
+            for (int k = 0; k < M; ++k) {
+                if (n == lane * V) {
+                    dt[k] += bias;
+                    if (a.softplus) dt[k] = softplus(dt[k]);
+                }
+                if (live[k]) {
+#pragma unroll
+                    for (int j = 0; j < V; ++j) {
+                        h[k].v[j] = power(dt[k] * w.v[j]) * h[k].v[j] + dt[k] * x[k] * widen(bb[k].v[j]);
+                        y[k] += widen(cc[k].v[j]) * h[k].v[j];
+                    }
+                }
+                if (here[k]) *(Pack<A, V>*)((A*)a.new_state + ((b0 + k) * a.d + c) * a.n + n) = h[k];
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < M; ++k) {
+            for (int o = lanes / 2; o > 0; o >>= 1) y[k] += __shfl_xor_sync(0xffffffffu, y[k], o);
+            if (!here[k] || lane) continue;
+            A v = y[k] + skip * x[k];
+            if (a.z) v *= gate(z[k]);
+            ((T*)a.y)[(b0 + k) * a.d + c] = narrow<T>(live[k] ? v : A(0));
         }
     }
-    for (int o = lanes / 2; o > 0; o >>= 1) y += __shfl_xor_sync(0xffffffffu, y, o);
-    if (!on || lane) return;
-    if (live) {
-        if (a.D) y += ((const A*)a.D)[c] * x;
-        if (a.z) y *= gate(widen(((const T*)a.z)[at]));
-    }
-    ((T*)a.y)[at] = narrow<T>(y);
+}
+
+template <typename T, int V>
+cudaError_t token(const SelectiveScanArgs& a, int lanes, int sm_count, cudaStream_t s) {
+    const int64_t across = (a.d * lanes + kThreads - 1) / kThreads;
+    if (across >= (1LL << 31)) return cudaErrorInvalidValue;
+    // four sequences at a time where that leaves two blocks for every SM
+    if (a.b >= 4 && across * ((a.b + 3) / 4) >= 2 * sm_count)
+        scan_token_kernel<T, V, 4><<<dim3((unsigned)across, (unsigned)std::min<int64_t>((a.b + 3) / 4, 65535)), kThreads, 0, s>>>(a, lanes);
+    else
+        scan_token_kernel<T, V, 1><<<dim3((unsigned)across, (unsigned)std::min<int64_t>(a.b, 65535)), kThreads, 0, s>>>(a, lanes);
+    return cudaGetLastError();
 }
 
 template <typename T>
-cudaError_t token(const SelectiveScanArgs& a, cudaStream_t s) {
+cudaError_t token(const SelectiveScanArgs& a, int sm_count, cudaStream_t s) {
     using A = typename Acc<T>::type;
     const int wide = sizeof(A) == 8 ? 2 : 4;
     const int v = a.n % wide == 0 ? wide : a.n % 2 == 0 ? 2 : 1;
     int lanes = 1;
     while (lanes < 32 && lanes * v < a.n) lanes *= 2;
-    const int64_t blocks = (a.b * a.d * lanes + kThreads - 1) / kThreads;
-    if (blocks >= (1LL << 31)) return cudaErrorInvalidValue;
-    if (v == 4) scan_token_kernel<T, 4><<<(unsigned)blocks, kThreads, 0, s>>>(a, lanes);
-    else if (v == 2) scan_token_kernel<T, 2><<<(unsigned)blocks, kThreads, 0, s>>>(a, lanes);
-    else scan_token_kernel<T, 1><<<(unsigned)blocks, kThreads, 0, s>>>(a, lanes);
-    return cudaGetLastError();
+    if (v == 4) return token<T, 4>(a, lanes, sm_count, s);
+    return v == 2 ? token<T, 2>(a, lanes, sm_count, s) : token<T, 1>(a, lanes, sm_count, s);
 }
 
 // ---- launches -------------------------------------------------------------------------------------------
@@ -633,7 +660,7 @@ cudaError_t prompt(const SelectiveScanArgs& a, int sm_count, cudaStream_t s) {
 
 template <typename T>
 cudaError_t scan(const SelectiveScanArgs& a, int sm_count, cudaStream_t s) {
-    if (a.t == 1) return token<T>(a, s);
+    if (a.t == 1) return token<T>(a, sm_count, s);
     if (a.n <= 8) return prompt<T, 4, 2>(a, sm_count, s);
     if (a.n <= 16) return prompt<T, 8, 2>(a, sm_count, s);
     if (a.n <= 32) return prompt<T, 8, 4>(a, sm_count, s);
