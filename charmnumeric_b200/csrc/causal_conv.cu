@@ -4,6 +4,10 @@
 //
 // X continues x to negative times with the state, the k - 1 inputs before the first.  The new state
 // is the last k - 1 rows of X; behind the end of a sequence y is 0.
+//
+// Bound by HBM: x is read and y written once.  A thread has V neighbouring channels (16 bytes where the
+// channels allow) and walks a run of steps with the last inputs in registers, so that an input is
+// loaded once but for the k - 1 in front of a run.
 #include <algorithm>
 
 #include "cn_types.hpp"
@@ -16,48 +20,139 @@ using namespace seq;
 
 namespace {
 
-template <typename T>
-__global__ void __launch_bounds__(256) causal_conv_kernel(CausalConvArgs a) {
+constexpr int kThreads = 128, kTogether = 4;    // steps whose inputs are requested together
+
+__device__ __forceinline__ float silu(float v) {
+    float e, r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(-1.4426950408889634f * v));
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + e));
+    return v * r;
+}
+__device__ __forceinline__ double silu(double v) { return v / (1.0 + exp(-v)); }
+
+// K is the width or more: filters are padded in front with zeros, over inputs that are zero there
+template <typename T, int V, int K>
+__global__ void __launch_bounds__(kThreads) causal_conv_kernel(CausalConvArgs a, int64_t run, int64_t runs) {
     using A = typename Acc<T>::type;
-    const int64_t c = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (c >= a.d) return;
-    for (int64_t b = blockIdx.z; b < a.b; b += gridDim.z) {
-    const int64_t end = a.lengths ? min(max((int64_t)a.lengths[b], (int64_t)0), a.t) : a.t;
-    const T* x = (const T*)a.x + b * a.t * a.d + c;
-    const T* st = a.state ? (const T*)a.state + b * (a.k - 1) * a.d + c : nullptr;
-    auto input = [&](int64_t t) -> T {
-        if (t >= 0) return x[t * a.d];
-        return st ? st[(t + a.k - 1) * a.d] : narrow<T>(A(0));
-    };
-    T* ns = (T*)a.new_state + b * (a.k - 1) * a.d + c;
-    T keep[kMaxConvWidth - 1];
-    if (blockIdx.y == 0)
-        for (int j = 0; j < a.k - 1; ++j) keep[j] = input(end - a.k + 1 + j);
-    for (int64_t t = blockIdx.y; t < a.t; t += gridDim.y) {
-        A s = a.bias ? widen(((const T*)a.bias)[c]) : A(0);
-        if (t < end) {
-            for (int j = 0; j < a.k; ++j) s += widen(((const T*)a.weight)[c * a.k + j]) * widen(input(t - a.k + 1 + j));
-            if (a.silu) s = s / (A(1) + exp(-s));
+    const int64_t id = (int64_t)blockIdx.x * kThreads + threadIdx.x, across = a.d / V;
+    if (id >= across * runs) return;
+    const int64_t c = id % across * V, t0 = id / across * run, t1 = min(t0 + run, a.t);
+    const int pad = K - a.k;
+    A w[K][V], bias[V];
+#pragma unroll
+    for (int j = 0; j < K; ++j)
+#pragma unroll
+        for (int v = 0; v < V; ++v) w[j][v] = j >= pad ? widen(((const T*)a.weight)[(c + v) * a.k + j - pad]) : A(0);
+#pragma unroll
+    for (int v = 0; v < V; ++v) bias[v] = a.bias ? widen(((const T*)a.bias)[c + v]) : A(0);
+    Pack<T, V> zero;
+#pragma unroll
+    for (int v = 0; v < V; ++v) zero.v[v] = narrow<T>(A(0));
+
+    for (int64_t b = blockIdx.y; b < a.b; b += gridDim.y) {
+        const int64_t end = a.lengths ? min(max((int64_t)a.lengths[b], (int64_t)0), a.t) : a.t;
+        const T* const xs = (const T*)a.x + b * a.t * a.d + c;
+        const T* const before = a.state ? (const T*)a.state + b * (a.k - 1) * a.d + c : nullptr;
+        T* const ys = (T*)a.y + b * a.t * a.d + c;
+        T* const after = (T*)a.new_state + b * (a.k - 1) * a.d + c;
+        auto input = [&](int64_t t) -> Pack<T, V> {
+            if (t >= 0) return *(const Pack<T, V>*)(xs + t * a.d);
+            return before && t + a.k - 1 >= 0 ? *(const Pack<T, V>*)(before + (t + a.k - 1) * a.d) : zero;
+        };
+        // the first run's threads carry the state: read before, written behind everything else, since
+        // it may be the same array for a single step
+        Pack<T, V> keep[K - 1];
+        if (t0 == 0) {
+#pragma unroll
+            for (int j = 0; j < K - 1; ++j)
+                if (j < a.k - 1) keep[j] = input(end - a.k + 1 + j);
         }
-        ((T*)a.y)[(b * a.t + t) * a.d + c] = t < end ? narrow<T>(s) : narrow<T>(A(0));
+        const int64_t live = min(t1, end);
+        int64_t t = t0;
+        if (t < live) {
+            A win[K - 1][V];
+#pragma unroll
+            for (int j = 0; j < K - 1; ++j) {
+                const Pack<T, V> p = input(t0 - K + 1 + j);
+#pragma unroll
+                for (int v = 0; v < V; ++v) win[j][v] = widen(p.v[v]);
+            }
+            auto step = [&](const Pack<T, V>& p, T* to) {
+                Pack<T, V> y;
+#pragma unroll
+                for (int v = 0; v < V; ++v) {
+                    const A x = widen(p.v[v]);
+                    A s = bias[v];
+#pragma unroll
+                    for (int j = 0; j < K - 1; ++j) s += w[j][v] * win[j][v];
+                    s += w[K - 1][v] * x;
+#pragma unroll
+                    for (int j = 0; j < K - 2; ++j) win[j][v] = win[j + 1][v];
+                    win[K - 2][v] = x;
+                    y.v[v] = narrow<T>(a.silu ? silu(s) : s);
+                }
+                *(Pack<T, V>*)to = y;
+            };
+            const T* from = xs + t * a.d;
+            T* to = ys + t * a.d;
+            for (; t + kTogether <= live; t += kTogether) {
+                Pack<T, V> p[kTogether];
+#pragma unroll
+                for (int i = 0; i < kTogether; ++i, from += a.d) p[i] = *(const Pack<T, V>*)from;
+#pragma unroll
+                for (int i = 0; i < kTogether; ++i, to += a.d) step(p[i], to);
+            }
+            for (; t < live; ++t, from += a.d, to += a.d) step(*(const Pack<T, V>*)from, to);
+        }
+        for (; t < t1; ++t) *(Pack<T, V>*)(ys + t * a.d) = zero;
+        if (t0 == 0) {
+#pragma unroll
+            for (int j = 0; j < K - 1; ++j)
+                if (j < a.k - 1) *(Pack<T, V>*)(after + j * a.d) = keep[j];
+        }
     }
-    if (blockIdx.y == 0)
-        for (int j = 0; j < a.k - 1; ++j) ns[j * a.d] = keep[j];
+}
+
+template <typename T, int V, int K>
+cudaError_t conv(const CausalConvArgs& a, int sm_count, cudaStream_t s) {
+    // Runs long enough that the k - 1 inputs in front of them are a small part (32 steps and more),
+    // as long as every SM has 16 warps; shorter ones down to 8 steps to get there
+    const int64_t across = a.d / V, threads = (int64_t)sm_count * 512;
+    int64_t run = 32;
+    while (run > 8 && across * a.b * ((a.t + run - 1) / run) < threads) run /= 2;
+    const int64_t runs = std::max<int64_t>((a.t + run - 1) / run, 1), blocks = (across * runs + kThreads - 1) / kThreads;
+    if (blocks >= (1LL << 31)) return cudaErrorInvalidValue;
+    causal_conv_kernel<T, V, K><<<dim3((unsigned)blocks, (unsigned)std::min<int64_t>(a.b, 65535)), kThreads, 0, s>>>(a, run, runs);
+    return cudaGetLastError();
+}
+
+template <typename T, int V>
+cudaError_t conv(const CausalConvArgs& a, int sm_count, cudaStream_t s) {
+    switch (a.k) {
+        case 2: return conv<T, V, 2>(a, sm_count, s);
+        case 3: return conv<T, V, 3>(a, sm_count, s);
+        case 4: return conv<T, V, 4>(a, sm_count, s);
+        default: return conv<T, V, kMaxConvWidth>(a, sm_count, s);
     }
+}
+
+template <typename T>
+cudaError_t conv(const CausalConvArgs& a, int sm_count, cudaStream_t s) {
+    constexpr int V = 16 / sizeof(T);
+    if (a.d % V == 0) return conv<T, V>(a, sm_count, s);
+    if (V > 2 && a.d % 2 == 0) return conv<T, 2>(a, sm_count, s);
+    return conv<T, 1>(a, sm_count, s);
 }
 
 }  // namespace
 
 cudaError_t launch_causal_conv(const CausalConvArgs& a, int sm_count, cudaStream_t s) {
-    (void)sm_count;
-    const dim3 grid((unsigned)((a.d + 255) / 256), (unsigned)std::max<int64_t>(1, std::min<int64_t>(a.t, 1024)), (unsigned)std::min<int64_t>(a.b, 65535));
     switch (a.dtype) {
-        case DT_F16: causal_conv_kernel<__half><<<grid, 256, 0, s>>>(a); break;
-        case DT_F32: causal_conv_kernel<float><<<grid, 256, 0, s>>>(a); break;
-        case DT_F64: causal_conv_kernel<double><<<grid, 256, 0, s>>>(a); break;
+        case DT_F16: return conv<__half>(a, sm_count, s);
+        case DT_F32: return conv<float>(a, sm_count, s);
+        case DT_F64: return conv<double>(a, sm_count, s);
         default: return cudaErrorInvalidValue;
     }
-    return cudaGetLastError();
 }
 
 }  // namespace cn

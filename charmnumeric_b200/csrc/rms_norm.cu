@@ -337,24 +337,56 @@ __device__ __forceinline__ To convert(From v) {
     else return (To)v;
 }
 
+// four values a thread and turn: one access of up to 16 (or two) bytes a value
 template <typename From, typename To>
 __global__ void __launch_bounds__(256) convert_kernel(const From* in, To* out, int64_t size) {
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < size; i += (int64_t)gridDim.x * 256)
-        out[i] = convert<To>(in[i]);
+    const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
+    if (i + 4 <= size) {
+        Pack<From, 4> v;
+        if constexpr (sizeof(From) == 8) {
+            *(Pack<From, 2>*)&v.v[0] = *(const Pack<From, 2>*)(in + i);
+            *(Pack<From, 2>*)&v.v[2] = *(const Pack<From, 2>*)(in + i + 2);
+        } else {
+            v = *(const Pack<From, 4>*)(in + i);
+        }
+        Pack<To, 4> w;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) w.v[j] = convert<To>(v.v[j]);
+        if constexpr (sizeof(To) == 8) {
+            *(Pack<To, 2>*)(out + i) = *(Pack<To, 2>*)&w.v[0];
+            *(Pack<To, 2>*)(out + i + 2) = *(Pack<To, 2>*)&w.v[2];
+        } else {
+            *(Pack<To, 4>*)(out + i) = w;
+        }
+    } else {
+        for (int64_t k = i; k < size; ++k) out[k] = convert<To>(in[k]);
+    }
 }
 
-template <typename To, typename S>
+// Values of codes: V neighbouring codes of a row and group a thread, rows down blockIdx.y; bound by HBM.
+template <typename To, typename S, int V>
 __global__ void __launch_bounds__(256)
 dequantize_kernel(const signed char* in, const S* scale, To* out, int64_t rows, int64_t n, int64_t group, int64_t groups) {
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < rows * n; i += (int64_t)gridDim.x * 256) {
-        const int64_t row = i / n, col = i - row * n;
-        out[i] = narrow<To>((typename Acc<To>::type)((S)in[i] * scale[row * groups + col / group]));
+    const int64_t col = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) * V;
+    if (col >= n) return;
+    const int64_t g = col / group;
+    for (int64_t row = (int64_t)blockIdx.y * blockDim.y + threadIdx.y; row < rows; row += (int64_t)gridDim.y * blockDim.y) {
+        const Pack<signed char, V> q = *(const Pack<signed char, V>*)(in + row * n + col);
+        const S f = scale[row * groups + g];
+        alignas(16) To v[V];
+#pragma unroll
+        for (int j = 0; j < V; ++j) v[j] = narrow<To>((typename Acc<To>::type)((S)q.v[j] * f));
+        constexpr int W = 16 / sizeof(To) < V ? 16 / sizeof(To) : V;
+#pragma unroll
+        for (int j = 0; j < V; j += W) *(Pack<To, W>*)(out + row * n + col + j) = *(Pack<To, W>*)&v[j];
     }
 }
 
 template <typename From>
-cudaError_t convert_from(const ConvertArgs& a, int grid, cudaStream_t s) {
-    const int64_t size = a.rows * a.n;
+cudaError_t convert_from(const ConvertArgs& a, cudaStream_t s) {
+    const int64_t size = a.rows * a.n, blocks = (size + 1023) / 1024;
+    if (blocks >= (1LL << 31)) return cudaErrorInvalidValue;
+    const unsigned grid = (unsigned)blocks;
     const From* in = (const From*)a.in;
     switch (a.to) {
         case DT_F32: convert_kernel<<<grid, 256, 0, s>>>(in, (float*)a.out, size); break;
@@ -368,14 +400,31 @@ cudaError_t convert_from(const ConvertArgs& a, int grid, cudaStream_t s) {
     return cudaGetLastError();
 }
 
-template <typename To>
-cudaError_t dequantize_to(const ConvertArgs& a, int grid, cudaStream_t s) {
-    const int64_t groups = (a.n + a.group - 1) / a.group;
-    if (a.scale_dtype == DT_F64)
-        dequantize_kernel<<<grid, 256, 0, s>>>((const signed char*)a.in, (const double*)a.scale, (To*)a.out, a.rows, a.n, a.group, groups);
-    else
-        dequantize_kernel<<<grid, 256, 0, s>>>((const signed char*)a.in, (const float*)a.scale, (To*)a.out, a.rows, a.n, a.group, groups);
+template <typename To, typename S, int V>
+cudaError_t dequantize(const ConvertArgs& a, int sm_count, cudaStream_t s) {
+    const int64_t groups = (a.n + a.group - 1) / a.group, pieces = (a.n + V - 1) / V;
+    int across = 32;
+    while (across < 256 && across < pieces) across *= 2;
+    const int down = 256 / across;
+    const int64_t bx = (pieces + across - 1) / across;
+    if (bx >= (1LL << 31)) return cudaErrorInvalidValue;
+    // enough blocks for 16 an SM, each over several rows
+    const int64_t by = std::max<int64_t>(1, std::min<int64_t>({(a.rows + down - 1) / down, (int64_t)sm_count * 16 / bx, 65535}));
+    dequantize_kernel<To, S, V><<<dim3((unsigned)bx, (unsigned)by), dim3(across, down), 0, s>>>(
+        (const signed char*)a.in, (const S*)a.scale, (To*)a.out, a.rows, a.n, a.group, groups);
     return cudaGetLastError();
+}
+
+template <typename To, typename S>
+cudaError_t dequantize(const ConvertArgs& a, int sm_count, cudaStream_t s) {
+    const bool whole = a.group >= a.n;
+    if (a.n % 8 == 0 && (whole || a.group % 8 == 0)) return dequantize<To, S, 8>(a, sm_count, s);
+    return dequantize<To, S, 1>(a, sm_count, s);
+}
+
+template <typename To>
+cudaError_t dequantize_to(const ConvertArgs& a, int sm_count, cudaStream_t s) {
+    return a.scale_dtype == DT_F64 ? dequantize<To, double>(a, sm_count, s) : dequantize<To, float>(a, sm_count, s);
 }
 
 }  // namespace
@@ -392,23 +441,22 @@ cudaError_t launch_rms_norm(const RmsNormArgs& a, int sm_count, cudaStream_t s) 
 }
 
 cudaError_t launch_convert(const ConvertArgs& a, int sm_count, cudaStream_t s) {
-    const int grid = (int)std::min<int64_t>((a.rows * a.n + 255) / 256, (int64_t)sm_count * 16);
-    if (grid < 1) return cudaSuccess;
+    if (a.rows * a.n < 1) return cudaSuccess;
     if (a.scale) {
         switch (a.to) {
-            case DT_F32: return dequantize_to<float>(a, grid, s);
-            case DT_F64: return dequantize_to<double>(a, grid, s);
-            case DT_F16: return dequantize_to<__half>(a, grid, s);
+            case DT_F32: return dequantize_to<float>(a, sm_count, s);
+            case DT_F64: return dequantize_to<double>(a, sm_count, s);
+            case DT_F16: return dequantize_to<__half>(a, sm_count, s);
             default: return cudaErrorInvalidValue;
         }
     }
     switch (a.from) {
-        case DT_F32: return convert_from<float>(a, grid, s);
-        case DT_F64: return convert_from<double>(a, grid, s);
-        case DT_I32: return convert_from<int>(a, grid, s);
-        case DT_I64: return convert_from<long long>(a, grid, s);
-        case DT_F16: return convert_from<__half>(a, grid, s);
-        case DT_I8: return convert_from<signed char>(a, grid, s);
+        case DT_F32: return convert_from<float>(a, s);
+        case DT_F64: return convert_from<double>(a, s);
+        case DT_I32: return convert_from<int>(a, s);
+        case DT_I64: return convert_from<long long>(a, s);
+        case DT_F16: return convert_from<__half>(a, s);
+        case DT_I8: return convert_from<signed char>(a, s);
         default: return cudaErrorInvalidValue;
     }
 }

@@ -511,10 +511,9 @@ __global__ void __launch_bounds__(kThreads + kHelpers, sizeof(T) <= 4 && N == 2 
 
 // ---- single tokens ------------------------------------------------------------------------------------
 //
-// The states are read and written once: a lane has V neighbouring states of a channel (16 bytes where n
-// allows), `lanes` lanes the channel, and M sequences at a time, whose loads are all on their way
-// before the first is used.  An inactive sequence's states are copied.
-template <typename T, int V, int M>
+// Bound by the states, which are read and written once: a lane has V neighbouring states of a channel
+// (16 bytes where n allows), `lanes` lanes the channel.  An inactive sequence's states are copied.
+template <typename T, int V>
 __global__ void __launch_bounds__(kThreads) scan_token_kernel(SelectiveScanArgs a, int lanes) {
     using A = typename Acc<T>::type;
     const int lane = threadIdx.x & (lanes - 1);
@@ -522,59 +521,98 @@ __global__ void __launch_bounds__(kThreads) scan_token_kernel(SelectiveScanArgs 
     const bool on = c < a.d;
     const int64_t bn = (int64_t)a.groups * a.n, g = on ? c / (a.d / a.groups) * a.n : 0;
     const A bias = on && a.delta_bias ? ((const A*)a.delta_bias)[c] : A(0), skip = on && a.D ? ((const A*)a.D)[c] : A(0);
-    for (int64_t b0 = (int64_t)blockIdx.y * M; b0 < a.b; b0 += (int64_t)gridDim.y * M) {
-        A x[M], dt[M], z[M], y[M];
-        bool here[M], live[M];
-#pragma unroll
-        for (int k = 0; k < M; ++k) {
-            const int64_t b = b0 + k;
-            here[k] = on && b < a.b;
-            live[k] = here[k] && !(a.lengths && a.lengths[b] < 1);
-            x[k] = live[k] ? widen(((const T*)a.x)[b * a.d + c]) : A(0);
-            dt[k] = live[k] ? widen(((const T*)a.delta)[b * a.d + c]) : A(0);
-            z[k] = live[k] && a.z ? widen(((const T*)a.z)[b * a.d + c]) : A(0);
-            y[k] = 0;
+    for (int64_t b = blockIdx.y; b < a.b; b += gridDim.y) {
+        const bool live = on && !(a.lengths && a.lengths[b] < 1);
+        const int64_t at = b * a.d + c;
+        A x = 0, dt = 0, out = 1, y = 0;
+        if (live) {
+            x = widen(((const T*)a.x)[at]);
+            dt = widen(((const T*)a.delta)[at]) + bias;
+            if (a.z) out = gate(widen(((const T*)a.z)[at]));
+            if (a.softplus) dt = softplus(dt);
         }
-        for (int n = lane * V; n < a.n; n += lanes * V) {
-            Pack<A, V> h[M], w;
-            Pack<T, V> bb[M], cc[M];
+        for (int n = lane * V; on && n < a.n; n += lanes * V) {
+            Pack<A, V> h;
 #pragma unroll
-            for (int j = 0; j < V; ++j) w.v[j] = on ? ((const A*)a.A)[c * a.n + n + j] * decay_scale<A>() : A(0);
+            for (int j = 0; j < V; ++j) h.v[j] = 0;
+            if (a.state) h = *(const Pack<A, V>*)((const A*)a.state + at * a.n + n);
+            if (live) {
+                const Pack<A, V> w = *(const Pack<A, V>*)((const A*)a.A + c * a.n + n);
+                const Pack<T, V> bb = *(const Pack<T, V>*)((const T*)a.B + b * bn + g + n), cc = *(const Pack<T, V>*)((const T*)a.C + b * bn + g + n);
 #pragma unroll
-            for (int k = 0; k < M; ++k) {
-                const int64_t b = b0 + k;
-#pragma unroll
-                for (int j = 0; j < V; ++j) h[k].v[j] = 0;
-                if (here[k] && a.state) h[k] = *(const Pack<A, V>*)((const A*)a.state + (b * a.d + c) * a.n + n);
-                if (live[k]) {
-                    bb[k] = *(const Pack<T, V>*)((const T*)a.B + b * bn + g + n);
-                    cc[k] = *(const Pack<T, V>*)((const T*)a.C + b * bn + g + n);
+                for (int j = 0; j < V; ++j) {
+                    h.v[j] = power(dt * (w.v[j] * decay_scale<A>())) * h.v[j] + dt * x * widen(bb.v[j]);
+                    y += widen(cc.v[j]) * h.v[j];
                 }
             }
+            *(Pack<A, V>*)((A*)a.new_state + at * a.n + n) = h;
+        }
+        for (int o = lanes / 2; o > 0; o >>= 1) y += __shfl_xor_sync(0xffffffffu, y, o);
+        if (on && lane == 0) ((T*)a.y)[at] = narrow<T>(live ? (y + skip * x) * out : A(0));
+    }
+}
+
+// Four sequences at a time, four or more lanes a channel: lane k of a channel computes dt, D x and the
+// gate of sequence k alone, hands dt and dt x to the others, and ends with the sum of that sequence.
+template <typename T, int V>
+__global__ void __launch_bounds__(kThreads) scan_tokens_kernel(SelectiveScanArgs a, int lanes) {
+    using A = typename Acc<T>::type;
+    const int lane = threadIdx.x & (lanes - 1), head = (threadIdx.x & 31) - lane, mine = lane & 3;
+    const int64_t c = ((int64_t)blockIdx.x * kThreads + threadIdx.x) / lanes;
+    const bool on = c < a.d;
+    const int64_t bn = (int64_t)a.groups * a.n, cn = on ? c * a.n : 0, g = on ? c / (a.d / a.groups) * a.n : 0, dn = a.d * a.n;
+    const A bias = on && a.delta_bias ? ((const A*)a.delta_bias)[c] : A(0), skip = on && a.D ? ((const A*)a.D)[c] : A(0);
+    for (int64_t b0 = (int64_t)blockIdx.y * 4; b0 < a.b; b0 += (int64_t)gridDim.y * 4) {
+        const int64_t b = b0 + mine;
+        const bool here = on && b < a.b, live = here && !(a.lengths && a.lengths[b] < 1);
+        A x = 0, dt = 0, out = 1, y[4] = {0, 0, 0, 0};
+        if (live) {
+            const int64_t at = b * a.d + c;
+            x = widen(((const T*)a.x)[at]);
+            dt = widen(((const T*)a.delta)[at]) + bias;
+            if (a.z) out = gate(widen(((const T*)a.z)[at]));
+            if (a.softplus) dt = softplus(dt);
+        }
+        const A dtx = dt * x;
+        const unsigned lives = __ballot_sync(0xffffffffu, live) >> head;
+        const T *bs = (const T*)a.B + b0 * bn + g, *cs = (const T*)a.C + b0 * bn + g;
+        const int64_t first = b0 * dn + cn;
+        for (int n0 = 0; n0 < a.n; n0 += lanes * V) {           // once, but for 128 states and more
+            const int n = n0 + lane * V;
+            const bool mid = on && n < a.n;
+            Pack<A, V> h[4], w;
+            Pack<T, V> bb[4], cc[4];
 #pragma unroll
-            for (int k = 0; k < M; ++k) {
-                if (n == lane * V) {
-                    dt[k] += bias;
-                    if (a.softplus) dt[k] = softplus(dt[k]);
+            for (int k = 0; k < 4; ++k) {
+#pragma unroll
+                for (int j = 0; j < V; ++j) h[k].v[j] = 0;
+                if (mid && b0 + k < a.b) {
+                    if (a.state) h[k] = *(const Pack<A, V>*)((const A*)a.state + first + k * dn + n);
+                    bb[k] = *(const Pack<T, V>*)(bs + k * bn + n);
+                    cc[k] = *(const Pack<T, V>*)(cs + k * bn + n);
                 }
-                if (live[k]) {
+            }
+            if (mid) w = *(const Pack<A, V>*)((const A*)a.A + cn + n);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const A dtk = __shfl_sync(0xffffffffu, dt, head + k), dtxk = __shfl_sync(0xffffffffu, dtx, head + k);
+                if (mid && lives >> k & 1) {
 #pragma unroll
                     for (int j = 0; j < V; ++j) {
-                        h[k].v[j] = power(dt[k] * w.v[j]) * h[k].v[j] + dt[k] * x[k] * widen(bb[k].v[j]);
+                        h[k].v[j] = power(dtk * (w.v[j] * decay_scale<A>())) * h[k].v[j] + dtxk * widen(bb[k].v[j]);
                         y[k] += widen(cc[k].v[j]) * h[k].v[j];
                     }
                 }
-                if (here[k]) *(Pack<A, V>*)((A*)a.new_state + ((b0 + k) * a.d + c) * a.n + n) = h[k];
+                if (mid && b0 + k < a.b) *(Pack<A, V>*)((A*)a.new_state + first + k * dn + n) = h[k];
             }
         }
-#pragma unroll
-        for (int k = 0; k < M; ++k) {
-            for (int o = lanes / 2; o > 0; o >>= 1) y[k] += __shfl_xor_sync(0xffffffffu, y[k], o);
-            if (!here[k] || lane) continue;
-            A v = y[k] + skip * x[k];
-            if (a.z) v *= gate(z[k]);
-            ((T*)a.y)[(b0 + k) * a.d + c] = narrow<T>(live[k] ? v : A(0));
-        }
+        // lanes at distance 2, then 1 exchange halves of the sequences; further lanes add theirs
+        const bool up2 = lane & 2, up1 = lane & 1;
+        A s0 = (up2 ? y[2] : y[0]) + __shfl_xor_sync(0xffffffffu, up2 ? y[0] : y[2], 2);
+        A s1 = (up2 ? y[3] : y[1]) + __shfl_xor_sync(0xffffffffu, up2 ? y[1] : y[3], 2);
+        A s = (up1 ? s1 : s0) + __shfl_xor_sync(0xffffffffu, up1 ? s0 : s1, 1);
+        for (int o = 4; o < lanes; o *= 2) s += __shfl_xor_sync(0xffffffffu, s, o);
+        if (here && lane < 4) ((T*)a.y)[b * a.d + c] = narrow<T>(live ? (s + skip * x) * out : A(0));
     }
 }
 
@@ -583,10 +621,11 @@ cudaError_t token(const SelectiveScanArgs& a, int lanes, int sm_count, cudaStrea
     const int64_t across = (a.d * lanes + kThreads - 1) / kThreads;
     if (across >= (1LL << 31)) return cudaErrorInvalidValue;
     // four sequences at a time where that leaves two blocks for every SM
-    if (a.b >= 4 && across * ((a.b + 3) / 4) >= 2 * sm_count)
-        scan_token_kernel<T, V, 4><<<dim3((unsigned)across, (unsigned)std::min<int64_t>((a.b + 3) / 4, 65535)), kThreads, 0, s>>>(a, lanes);
+    const dim3 fours((unsigned)across, (unsigned)std::min<int64_t>((a.b + 3) / 4, 65535));
+    if (a.b >= 4 && lanes >= 4 && across * ((a.b + 3) / 4) >= 2 * sm_count)
+        scan_tokens_kernel<T, V><<<fours, kThreads, 0, s>>>(a, lanes);
     else
-        scan_token_kernel<T, V, 1><<<dim3((unsigned)across, (unsigned)std::min<int64_t>(a.b, 65535)), kThreads, 0, s>>>(a, lanes);
+        scan_token_kernel<T, V><<<dim3((unsigned)across, (unsigned)std::min<int64_t>(a.b, 65535)), kThreads, 0, s>>>(a, lanes);
     return cudaGetLastError();
 }
 
