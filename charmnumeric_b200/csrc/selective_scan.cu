@@ -552,67 +552,74 @@ __global__ void __launch_bounds__(kThreads) scan_token_kernel(SelectiveScanArgs 
     }
 }
 
-// Four sequences at a time, four or more lanes a channel: lane k of a channel computes dt, D x and the
-// gate of sequence k alone, hands dt and dt x to the others, and ends with the sum of that sequence.
+// Runs of sequences, four at a time, with four or more lanes a channel that have all of its states:
+// lane k of a channel computes dt, D x and the gate of sequence k alone, hands dt and dt x to the others,
+// and ends with the sum of that sequence.  Addresses are stepped from sequence to sequence.
 template <typename T, int V>
-__global__ void __launch_bounds__(kThreads) scan_tokens_kernel(SelectiveScanArgs a, int lanes) {
+__global__ void __launch_bounds__(kThreads, 3) scan_tokens_kernel(SelectiveScanArgs a, int lanes, int run) {
     using A = typename Acc<T>::type;
-    const int lane = threadIdx.x & (lanes - 1), head = (threadIdx.x & 31) - lane, mine = lane & 3;
+    const int lane = threadIdx.x & (lanes - 1), head = (threadIdx.x & 31) - lane, mine = lane & 3, n = lane * V;
     const int64_t c = ((int64_t)blockIdx.x * kThreads + threadIdx.x) / lanes;
-    const bool on = c < a.d;
-    const int64_t bn = (int64_t)a.groups * a.n, cn = on ? c * a.n : 0, g = on ? c / (a.d / a.groups) * a.n : 0, dn = a.d * a.n;
+    const bool on = c < a.d, mid = on && n < a.n;
+    const int64_t bn = (int64_t)a.groups * a.n, dn = a.d * a.n;
+    const int64_t b0 = (int64_t)blockIdx.y * run, b1 = min(b0 + run, a.b);
     const A bias = on && a.delta_bias ? ((const A*)a.delta_bias)[c] : A(0), skip = on && a.D ? ((const A*)a.D)[c] : A(0);
-    for (int64_t b0 = (int64_t)blockIdx.y * 4; b0 < a.b; b0 += (int64_t)gridDim.y * 4) {
-        const int64_t b = b0 + mine;
-        const bool here = on && b < a.b, live = here && !(a.lengths && a.lengths[b] < 1);
-        A x = 0, dt = 0, out = 1, y[4] = {0, 0, 0, 0};
+    Pack<A, V> w;
+#pragma unroll
+    for (int j = 0; j < V; ++j) w.v[j] = mid ? ((const A*)a.A)[c * a.n + n + j] * decay_scale<A>() : A(0);
+    const int64_t first = mid ? b0 * dn + c * a.n + n : 0;
+    const A* hs = (const A*)a.state + first;
+    A* hn = (A*)a.new_state + first;
+    const int64_t first_b = mid ? b0 * bn + c / (a.d / a.groups) * a.n + n : 0;
+    const T *bs = (const T*)a.B + first_b, *cs = (const T*)a.C + first_b;
+    int64_t at = (b0 + mine) * a.d + (on ? c : 0);
+    for (int64_t b = b0; b < b1; b += 4, at += 4 * a.d) {
+        const int here = (int)min(b1 - b, (int64_t)4);
+        Pack<A, V> h[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+#pragma unroll
+            for (int j = 0; j < V; ++j) h[k].v[j] = 0;
+            if (mid && k < here && a.state) h[k] = *(const Pack<A, V>*)hs;
+            hs += dn;
+        }
+        const bool live = on && mine < here && !(a.lengths && a.lengths[b + mine] < 1);
+        A x = 0, dt = 0, z = 0, y[4] = {0, 0, 0, 0};
         if (live) {
-            const int64_t at = b * a.d + c;
             x = widen(((const T*)a.x)[at]);
             dt = widen(((const T*)a.delta)[at]) + bias;
-            if (a.z) out = gate(widen(((const T*)a.z)[at]));
+            if (a.z) z = widen(((const T*)a.z)[at]);
             if (a.softplus) dt = softplus(dt);
         }
         const A dtx = dt * x;
         const unsigned lives = __ballot_sync(0xffffffffu, live) >> head;
-        const T *bs = (const T*)a.B + b0 * bn + g, *cs = (const T*)a.C + b0 * bn + g;
-        const int64_t first = b0 * dn + cn;
-        for (int n0 = 0; n0 < a.n; n0 += lanes * V) {           // once, but for 128 states and more
-            const int n = n0 + lane * V;
-            const bool mid = on && n < a.n;
-            Pack<A, V> h[4], w;
-            Pack<T, V> bb[4], cc[4];
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
+        for (int k = 0; k < 4; ++k) {
+            const A dtk = __shfl_sync(0xffffffffu, dt, head + k), dtxk = __shfl_sync(0xffffffffu, dtx, head + k);
+            if (mid && lives >> k & 1) {
+                const Pack<T, V> bb = *(const Pack<T, V>*)bs, cc = *(const Pack<T, V>*)cs;
 #pragma unroll
-                for (int j = 0; j < V; ++j) h[k].v[j] = 0;
-                if (mid && b0 + k < a.b) {
-                    if (a.state) h[k] = *(const Pack<A, V>*)((const A*)a.state + first + k * dn + n);
-                    bb[k] = *(const Pack<T, V>*)(bs + k * bn + n);
-                    cc[k] = *(const Pack<T, V>*)(cs + k * bn + n);
+                for (int j = 0; j < V; ++j) {
+                    h[k].v[j] = power(dtk * w.v[j]) * h[k].v[j] + dtxk * widen(bb.v[j]);
+                    y[k] += widen(cc.v[j]) * h[k].v[j];
                 }
             }
-            if (mid) w = *(const Pack<A, V>*)((const A*)a.A + cn + n);
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                const A dtk = __shfl_sync(0xffffffffu, dt, head + k), dtxk = __shfl_sync(0xffffffffu, dtx, head + k);
-                if (mid && lives >> k & 1) {
-#pragma unroll
-                    for (int j = 0; j < V; ++j) {
-                        h[k].v[j] = power(dtk * (w.v[j] * decay_scale<A>())) * h[k].v[j] + dtxk * widen(bb[k].v[j]);
-                        y[k] += widen(cc[k].v[j]) * h[k].v[j];
-                    }
-                }
-                if (mid && b0 + k < a.b) *(Pack<A, V>*)((A*)a.new_state + first + k * dn + n) = h[k];
-            }
+            if (mid && k < here) *(Pack<A, V>*)hn = h[k];
+            hn += dn;
+            bs += bn;
+            cs += bn;
         }
         // lanes at distance 2, then 1 exchange halves of the sequences; further lanes add theirs
         const bool up2 = lane & 2, up1 = lane & 1;
-        A s0 = (up2 ? y[2] : y[0]) + __shfl_xor_sync(0xffffffffu, up2 ? y[0] : y[2], 2);
-        A s1 = (up2 ? y[3] : y[1]) + __shfl_xor_sync(0xffffffffu, up2 ? y[1] : y[3], 2);
+        const A s0 = (up2 ? y[2] : y[0]) + __shfl_xor_sync(0xffffffffu, up2 ? y[0] : y[2], 2);
+        const A s1 = (up2 ? y[3] : y[1]) + __shfl_xor_sync(0xffffffffu, up2 ? y[1] : y[3], 2);
         A s = (up1 ? s1 : s0) + __shfl_xor_sync(0xffffffffu, up1 ? s0 : s1, 1);
         for (int o = 4; o < lanes; o *= 2) s += __shfl_xor_sync(0xffffffffu, s, o);
-        if (here && lane < 4) ((T*)a.y)[b * a.d + c] = narrow<T>(live ? (s + skip * x) * out : A(0));
+        if (on && mine < here && lane < 4) {
+            s += skip * x;
+            if (a.z) s *= gate(z);
+            ((T*)a.y)[at] = narrow<T>(live ? s : A(0));
+        }
     }
 }
 
@@ -620,10 +627,12 @@ template <typename T, int V>
 cudaError_t token(const SelectiveScanArgs& a, int lanes, int sm_count, cudaStream_t s) {
     const int64_t across = (a.d * lanes + kThreads - 1) / kThreads;
     if (across >= (1LL << 31)) return cudaErrorInvalidValue;
-    // four sequences at a time where that leaves two blocks for every SM
-    const dim3 fours((unsigned)across, (unsigned)std::min<int64_t>((a.b + 3) / 4, 65535));
-    if (a.b >= 4 && lanes >= 4 && across * ((a.b + 3) / 4) >= 2 * sm_count)
-        scan_tokens_kernel<T, V><<<fours, kThreads, 0, s>>>(a, lanes);
+    // runs of up to 16 sequences, as long as four blocks for every SM are left; else one by one
+    int64_t run = 16;
+    while (run > 4 && across * ((a.b + run - 1) / run) < 4 * sm_count) run /= 2;
+    const int64_t runs = (a.b + run - 1) / run;
+    if (a.b >= 4 && lanes >= 4 && lanes * V >= a.n && across * runs >= 2 * sm_count && runs <= 65535)
+        scan_tokens_kernel<T, V><<<dim3((unsigned)across, (unsigned)runs), kThreads, 0, s>>>(a, lanes, (int)run);
     else
         scan_token_kernel<T, V><<<dim3((unsigned)across, (unsigned)std::min<int64_t>(a.b, 65535)), kThreads, 0, s>>>(a, lanes);
     return cudaGetLastError();
