@@ -101,7 +101,7 @@ def sample_row(x, u, temperature, top_k, top_p, min_p):
     if not temperature > 0:
         return int(x.argmax()), 0.0
     with np.errstate(invalid="ignore"):
-        z = np.where(x == most, 0.0, np.where(x == -np.inf, -np.inf, (x - most) / temperature))
+        z = np.where(x == most, 0.0, np.where((x == -np.inf) | (most == np.inf), -np.inf, (x * 0.5 - most * 0.5) / temperature * 2.0))  # halves: no overflow
     e = np.exp(z)
     keep = np.argsort(-x, kind="stable")
     if 1 <= top_k < len(x):

@@ -341,7 +341,7 @@ def logp_bound(x, temperature, dtype):
     """Errors of a weight: its argument's rounding and the exponential's (relative)."""
     most = x.max()
     with np.errstate(all="ignore"):
-        z = np.where(x == most, 0.0, np.where(np.isfinite(most), np.maximum((x - most) / max(temperature, 1e-30), -700.0), -700.0))
+        z = np.where(x == most, 0.0, np.where(np.isfinite(most), np.maximum((x * 0.5 - most * 0.5) / max(temperature, 1e-30) * 2.0, -700.0), -700.0))
     e = np.exp(z)
     return unit(dtype) * float((e * (3 * np.abs(z) + 8)).sum() / e.sum()) * 2 + 2.0 ** -36
 
@@ -441,6 +441,22 @@ def test_sample_masks_ties_and_infinities(interface, v, dtype):
         assert gpu[f"t{i}"][0] == -1 and gpu[f"t{i}"][1] == -1
 
 
+@pytest.mark.parametrize("dtype,v", [("float16", 600000), ("float32", 262145), ("float32", 1000003), ("float64", 300000)])
+def test_sample_vocabularies_beyond_shared_memory(interface, dtype, v):
+    rng = np.random.default_rng(v)
+    x = (rng.standard_normal((2, v)) * 2).astype(dtype)
+    u = np.array([0.3, 0.999], "float64" if dtype == "float64" else "float32")
+    sets = [(1.0, 0, 1.0, 0.0), (0.8, 300, 0.9, 0.0), (1.5, 0, 0.97, 0.001)]
+    def program():
+        out, ax, au = {}, cnp.asarray(x), cnp.asarray(u)
+        for i, (t, k, p, m) in enumerate(sets):
+            out[f"t{i}"], out[f"p{i}"] = cnp.random.sample(ax, au, temperature=t, top_k=k, top_p=p, min_p=m)
+        return out
+    gpu, _ = run_both(interface, program)
+    for i, f in enumerate(sets):
+        check_samples(x, gpu[f"t{i}"], gpu[f"p{i}"], u, *f)
+
+
 def test_sample_one_dimension_and_given_numbers(interface):
     rng = np.random.default_rng(1)
     x = rng.standard_normal(3000)
@@ -460,6 +476,26 @@ def test_sample_frequencies(interface):
     gpu, _ = run_both(interface, lambda: {"t": cnp.random.sample(cnp.asarray(x), cnp.random.uniform((rows,), seed=3))[0]})
     counts = np.bincount(gpu["t"], minlength=5)
     assert (np.abs(counts - rows * p) <= 5 * np.sqrt(rows * p * (1 - p))).all(), counts
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_sample_extreme_temperatures_and_spans(interface, dtype):
+    """Weights that are all alike, all but one nothing, and logits at both ends of the type."""
+    rng = np.random.default_rng(21)
+    big = float(np.finfo(dtype).max)
+    v = 9000
+    x = np.stack([rng.standard_normal(v), np.linspace(-big, big, v), np.where(np.arange(v) % 7, -big, big * 0.5),
+                  rng.standard_normal(v) * 1e-3, 20 + rng.standard_normal(v) * 1e-2, np.where(np.arange(v) == 4000, 60.0, rng.standard_normal(v))]).astype(dtype)
+    u = np.array([0.1, 0.3, 0.5, 0.7, 0.9, 0.99999], "float32")
+    sets = [(t, k, p, 0.0) for t in (1e-30, 1e-3, 1.0, 1e4, 1e30, float("inf")) for k, p in ((0, 0.7), (100, 1.0), (4500, 0.5))]
+    def program():
+        out, ax, au = {}, cnp.asarray(x), cnp.asarray(u)
+        for i, (t, k, p, m) in enumerate(sets):
+            out[f"t{i}"], out[f"p{i}"] = cnp.random.sample(ax, au, temperature=t, top_k=k, top_p=p, min_p=m)
+        return out
+    gpu, _ = run_both(interface, program)
+    for i, f in enumerate(sets):
+        check_samples(x, gpu[f"t{i}"], gpu[f"p{i}"], u, *f)
 
 
 # ---- conversions, storage types, steps ----------------------------------------------------------------------------
