@@ -95,12 +95,21 @@ __device__ __forceinline__ double power(double v) { return exp2(v); }
 // Weights e of 0 to 1 as integers.  WIDE: 64 bits at once, rint(e 2^shift).  Else three limbs of 15 bits,
 // whose sums over a slice of up to 2^15 values fit the 32 bits that shared memory can add to at once,
 // and whose sum over 8 slices fits 64.
+// A histogram is an array of bins of 64 bits, or three arrays of the limbs' sums.
 template <bool WIDE> struct Mass;
 template <> struct Mass<true> {
     static constexpr int kWords = 2;
     template <typename A> __device__ static u64 of(A e, int shift) { return (u64)rint(e * (A)(1ULL << shift)); }
-    template <typename A> __device__ static void add(unsigned* bin, A e, int shift) { atomicAdd((u64*)bin, of(e, shift)); }
-    __device__ static u64 read(const unsigned* bin) { return *(const u64*)bin; }
+    template <typename A> __device__ static void add(unsigned* bins, int bin, A e, int shift) { atomicAdd((u64*)bins + bin, of(e, shift)); }
+    __device__ static void count(unsigned* bins, int bin) { atomicAdd((u64*)bins + bin, 1ULL); }
+    // bins 2 i and 2 i + 1, summed over the blocks; every block begins with its own
+    template <bool COUNT, typename F> __device__ static void sum(u64 (&own)[2], int i, int blocks, F&& bins_of) {
+        for (int q = 0; q < blocks; ++q) {
+            const Pack<u64, 2> w = ((const Pack<u64, 2>*)bins_of(q))[i];
+            own[0] += w.v[0];
+            own[1] += w.v[1];
+        }
+    }
 };
 template <> struct Mass<false> {
     static constexpr int kWords = 3;
@@ -117,19 +126,39 @@ template <> struct Mass<false> {
         limbs(e, l);
         return ((u64)l[0] << 30) + ((u64)l[1] << 15) + l[2];
     }
-    __device__ static void add(unsigned* bin, float e, int) {
+    __device__ static void add(unsigned* bins, int bin, float e, int) {
         unsigned l[3];
         limbs(e, l);
-        if (l[0]) atomicAdd(bin, l[0]);
-        if (l[1]) atomicAdd(bin + 1, l[1]);
-        if (l[2]) atomicAdd(bin + 2, l[2]);
+        if (l[0]) atomicAdd(bins + bin, l[0]);
+        if (l[1]) atomicAdd(bins + kBins + bin, l[1]);
+        if (l[2]) atomicAdd(bins + 2 * kBins + bin, l[2]);
     }
-    __device__ static u64 read(const unsigned* bin) { return ((u64)bin[0] << 30) + ((u64)bin[1] << 15) + bin[2]; }
+    __device__ static void count(unsigned* bins, int bin) { atomicAdd(bins + 2 * kBins + bin, 1u); }
+    template <bool COUNT, typename F> __device__ static void sum(u64 (&own)[2], int i, int blocks, F&& bins_of) {
+#pragma unroll
+        for (int k = COUNT ? 2 : 0; k < 3; ++k) {
+            // all blocks' values are on their way before the first is added
+            Pack<unsigned, 2> w[kMostBlocks];
+#pragma unroll
+            for (int q = 0; q < kMostBlocks; ++q) {
+                if (q < blocks) w[q] = ((const Pack<unsigned, 2>*)(bins_of(q) + k * kBins))[i];
+                else w[q] = {{0, 0}};
+            }
+            u64 a = 0, b = 0;
+#pragma unroll
+            for (int q = 0; q < kMostBlocks; ++q) {
+                a += w[q].v[0];
+                b += w[q].v[1];
+            }
+            own[0] += a << 15 * (2 - k);
+            own[1] += b << 15 * (2 - k);
+        }
+    }
 };
 
 template <typename T, bool WIDE>
 struct SampleShared {
-    alignas(16) unsigned bins[2][kBins][Mass<WIDE>::kWords];   // two rounds' histograms
+    alignas(16) unsigned bins[2][kBins * Mass<WIDE>::kWords];  // two rounds' histograms
     u64 scan[kWarps];
     u64 weight[kWarps];                                        // each warp's kept weight above the border
     u64 tied[kWarps];                                          // ... and values at the border
@@ -211,7 +240,7 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(SampleArgs a, int64_t 
     } else {
         each([&](Key k) { top = k > top ? k : top; });
     }
-    for (int i = tid; i < 2 * kBins * M::kWords; i += kThreads) (&sh.bins[0][0][0])[i] = 0;
+    for (int i = tid; i < 2 * kBins * M::kWords; i += kThreads) (&sh.bins[0][0])[i] = 0;
     top = warp_max(top);
     if (lane == 0) sh.top[warp] = top;
     __syncthreads();
@@ -221,10 +250,8 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(SampleArgs a, int64_t 
     }
     cluster.sync();
     top = 0;
-    for (int q = 0; q < blocks; ++q) {
-        const Key k = *cluster.map_shared_rank(&sh.most, q);
-        top = k > top ? k : top;
-    }
+    if (lane < blocks) top = *cluster.map_shared_rank(&sh.most, lane);
+    top = warp_max(top);
     const A most = O::value(top);
     const A temp = (A)row_param(a.temperature, row);
     const bool none = most == -INFINITY, greedy = !(temp > 0), alone = greedy || most == INFINITY;
@@ -256,7 +283,7 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(SampleArgs a, int64_t 
         u64 above = 0, target = 0;
         // a round leaves 1/1024 of the span or less: 8 are the most for 64-bit keys
         for (int round = 0; round < 12; ++round) {
-            unsigned (*bins)[M::kWords] = sh.bins[turn & 1];
+            unsigned* const bins = sh.bins[turn & 1];
             each([&](Key k) {
                 if (k < edge || k < low || k > high) return;
                 int bin;
@@ -266,16 +293,12 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(SampleArgs a, int64_t 
                     if (octave_bin(k) != octave) return;
                     bin = (int)((high - k) >> down);
                 }
-                if (kWeight) M::add(bins[bin], weight(k), shift);
-                else atomicAdd(&bins[bin][0], 1u);
+                if (kWeight) M::add(bins, bin, weight(k), shift);
+                else M::count(bins, bin);
             });
             cluster.sync();
             u64 own[2] = {0, 0};
-            for (int q = 0; q < blocks; ++q) {
-                const unsigned (*theirs)[M::kWords] = cluster.map_shared_rank(bins, q);
-#pragma unroll
-                for (int i = 0; i < 2; ++i) own[i] += kWeight ? M::read(theirs[2 * tid + i]) : (u64)theirs[2 * tid + i][0];
-            }
+            M::template sum<!kWeight>(own, tid, blocks, [&](int q) { return cluster.map_shared_rank(bins, (rank + q) & (blocks - 1)); });
             if (tid == 0) sh.found = -1;
             u64 total;
             u64 before = above + block_prefix(own[0] + own[1], sh.scan, &total);
@@ -291,7 +314,7 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(SampleArgs a, int64_t 
             }
             // the other histogram is free: all blocks have passed the barrier behind its last use
             ++turn;
-            for (int i = tid; i < kBins * M::kWords; i += kThreads) (&sh.bins[turn & 1][0][0])[i] = 0;
+            for (int i = tid; i < kBins * M::kWords; i += kThreads) sh.bins[turn & 1][i] = 0;
             __syncthreads();
             const int found = sh.found;
             if (found < 0) break;
