@@ -15,8 +15,8 @@
 //
 // Nothing is sorted.  A cluster of up to 8 blocks has a row, each block a slice of it in shared memory as
 // integer keys in the order of the values, read from HBM once.  A border is found by histograms: the
-// first over steps of 1/32 in log2 e, the next over what the bin with the border spans in key space,
-// 1024 times finer each time, until a bin is one key.  Every block adds up all blocks' histograms
+// first over steps of 1/16 in log2 e, the next over what the bin with the border spans in key space,
+// 512 times finer each time, until a bin is one key.  Every block adds up all blocks' histograms
 // (distributed shared memory), so that one cluster barrier a round is enough.
 #include <cooperative_groups.h>
 
@@ -35,8 +35,8 @@ namespace {
 
 typedef unsigned long long u64;
 
-constexpr int kThreads = 512, kWarps = kThreads / 32, kBins = 2 * kThreads, kMostBlocks = 8;
-constexpr int kBinsPerOctave = 32;
+constexpr int kThreads = 512, kWarps = kThreads / 32, kBins = kThreads, kMostBlocks = 8;
+constexpr int kBinsPerOctave = 16, kGrain = 256;
 
 // Integers in the order of the values; -0 and 0 are one value, NaN the lowest.
 template <typename T> struct Order;
@@ -79,6 +79,38 @@ template <> struct Order<double> {
     __device__ static Key at_most(double x) { const Key k = key(x); return k ? k - 1 : 0; }
 };
 
+// Keys of V neighbouring values.  16-bit values two at a time: a value's sign decides whether all of its
+// bits or the sign alone are turned; NaN and -0 are left to the single value's routine.
+template <typename T, int V>
+__device__ __forceinline__ Pack<typename Order<T>::Stored, V> keys_of(const Pack<T, V>& p) {
+    Pack<typename Order<T>::Stored, V> q;
+    if constexpr (sizeof(T) == 2 && V % 2 == 0) {
+        Pack<unsigned, V / 2> u = *(const Pack<unsigned, V / 2>*)&p;
+        unsigned odd = 0;
+#pragma unroll
+        for (int j = 0; j < V / 2; ++j) {
+            const unsigned w = u.v[j];
+            odd |= __vcmpgtu2(w & 0x7fff7fffu, 0x7c007c00u) | __vcmpeq2(w, 0x80008000u);
+            u.v[j] = w ^ ((w >> 15 & 0x00010001u) * 0x7fffu | 0x80008000u);
+        }
+        if (!odd) return *(const Pack<unsigned short, V>*)&u;
+    }
+#pragma unroll
+    for (int j = 0; j < V; ++j) q.v[j] = (typename Order<T>::Stored)Order<T>::key(p.v[j]);
+    return q;
+}
+
+// whether any key of a piece is at least `from`
+__device__ __forceinline__ bool any_from(const Pack<unsigned short, 8>& q, unsigned from) {
+    const Pack<unsigned, 4> u = *(const Pack<unsigned, 4>*)&q;
+    const unsigned both = from * 0x10001u;
+    return __vcmpgeu2(u.v[0], both) | __vcmpgeu2(u.v[1], both) | __vcmpgeu2(u.v[2], both) | __vcmpgeu2(u.v[3], both);
+}
+__device__ __forceinline__ bool any_from(const Pack<unsigned, 4>& q, unsigned from) {
+    return max(max(q.v[0], q.v[1]), max(q.v[2], q.v[3])) >= from;
+}
+__device__ __forceinline__ bool any_from(const Pack<u64, 2>& q, u64 from) { return q.v[0] >= from || q.v[1] >= from; }
+
 __device__ __forceinline__ double row_param(const RowParam& p, int64_t row) {
     if (!p.data) return p.value;
     if (p.dtype == DT_I32) return (double)((const int*)p.data)[row];
@@ -102,57 +134,45 @@ template <> struct Mass<true> {
     template <typename A> __device__ static u64 of(A e, int shift) { return (u64)rint(e * (A)(1ULL << shift)); }
     template <typename A> __device__ static void add(unsigned* bins, int bin, A e, int shift) { atomicAdd((u64*)bins + bin, of(e, shift)); }
     __device__ static void count(unsigned* bins, int bin) { atomicAdd((u64*)bins + bin, 1ULL); }
-    // bins 2 i and 2 i + 1, summed over the blocks; every block begins with its own
-    template <bool COUNT, typename F> __device__ static void sum(u64 (&own)[2], int i, int blocks, F&& bins_of) {
-        for (int q = 0; q < blocks; ++q) {
-            const Pack<u64, 2> w = ((const Pack<u64, 2>*)bins_of(q))[i];
-            own[0] += w.v[0];
-            own[1] += w.v[1];
-        }
+    // bin i, summed over the blocks
+    template <bool COUNT, typename F> __device__ static u64 sum(int i, int blocks, F&& bins_of) {
+        u64 own = 0;
+        for (int q = 0; q < blocks; ++q) own += ((const u64*)bins_of(q))[i];
+        return own;
     }
 };
 template <> struct Mass<false> {
     static constexpr int kWords = 3;
-    __device__ static void limbs(float e, unsigned (&l)[3]) {
-        // every difference and product is exact
-        const float s = e * 32768.0f;
-        l[0] = (unsigned)s;
-        const float t = (s - (float)l[0]) * 32768.0f;
-        l[1] = (unsigned)t;
-        l[2] = (unsigned)rintf((t - (float)l[1]) * 32768.0f);
-    }
+    // e 2^45 to the nearest: the significand shifted by the exponent, without a conversion's slow unit
     __device__ static u64 of(float e, int) {
-        unsigned l[3];
-        limbs(e, l);
-        return ((u64)l[0] << 30) + ((u64)l[1] << 15) + l[2];
+        const unsigned bits = __float_as_uint(e), significand = (bits & 0x7fffffu) | 0x800000u;
+        const int up = (int)(bits >> 23) - 105;       // 1 is 2^23 2^22
+        if (up >= 0) return (u64)significand << up;
+        return up > -26 ? (significand + (1u << (-up - 1))) >> -up : 0;
     }
     __device__ static void add(unsigned* bins, int bin, float e, int) {
-        unsigned l[3];
-        limbs(e, l);
-        if (l[0]) atomicAdd(bins + bin, l[0]);
-        if (l[1]) atomicAdd(bins + kBins + bin, l[1]);
-        if (l[2]) atomicAdd(bins + 2 * kBins + bin, l[2]);
+        const u64 m = of(e, 0);
+        if (m >> 30) atomicAdd(bins + bin, (unsigned)(m >> 30));     // the largest few
+        atomicAdd(bins + kBins + bin, (unsigned)(m >> 15) & 0x7fffu);
+        atomicAdd(bins + 2 * kBins + bin, (unsigned)m & 0x7fffu);
     }
     __device__ static void count(unsigned* bins, int bin) { atomicAdd(bins + 2 * kBins + bin, 1u); }
-    template <bool COUNT, typename F> __device__ static void sum(u64 (&own)[2], int i, int blocks, F&& bins_of) {
+    template <bool COUNT, typename F> __device__ static u64 sum(int i, int blocks, F&& bins_of) {
+        // all blocks' values are on their way before the first is added
+        unsigned w[COUNT ? 1 : 3][kMostBlocks];
 #pragma unroll
-        for (int k = COUNT ? 2 : 0; k < 3; ++k) {
-            // all blocks' values are on their way before the first is added
-            Pack<unsigned, 2> w[kMostBlocks];
+        for (int q = 0; q < kMostBlocks; ++q)
 #pragma unroll
-            for (int q = 0; q < kMostBlocks; ++q) {
-                if (q < blocks) w[q] = ((const Pack<unsigned, 2>*)(bins_of(q) + k * kBins))[i];
-                else w[q] = {{0, 0}};
-            }
-            u64 a = 0, b = 0;
+            for (int k = 0; k < (COUNT ? 1 : 3); ++k) w[k][q] = q < blocks ? bins_of(q)[(COUNT ? 2 : k) * kBins + i] : 0;
+        u64 own = 0;
 #pragma unroll
-            for (int q = 0; q < kMostBlocks; ++q) {
-                a += w[q].v[0];
-                b += w[q].v[1];
-            }
-            own[0] += a << 15 * (2 - k);
-            own[1] += b << 15 * (2 - k);
+        for (int k = 0; k < (COUNT ? 1 : 3); ++k) {
+            u64 limb = 0;
+#pragma unroll
+            for (int q = 0; q < kMostBlocks; ++q) limb += w[k][q];
+            own += COUNT ? limb : limb << 15 * (2 - k);
         }
+        return own;
     }
 };
 
@@ -191,9 +211,9 @@ __device__ __forceinline__ u64 block_prefix(u64 v, u64* sm, u64* total) {
 }
 
 // One cluster a row.  RESIDENT: a block's slice fits its shared memory; else it is read from L2 each time.
-// V: values of one load.  A warp has `per_warp` neighbouring values (a multiple of 32) of the slice.
+// V: values of one load.  A warp has `per_warp` neighbouring values (a multiple of kGrain) of the slice.
 template <typename T, int V, bool WIDE, bool RESIDENT>
-__global__ void __launch_bounds__(kThreads) sample_kernel(SampleArgs a, int64_t per_warp, int shift) {
+__global__ void __launch_bounds__(kThreads, sizeof(T) == 8 ? 1 : 2) sample_kernel(SampleArgs a, int64_t per_warp, int shift) {
     using A = typename Acc<T>::type;
     using O = Order<T>;
     using Key = typename O::Key;
@@ -205,42 +225,61 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(SampleArgs a, int64_t 
     cg::cluster_group cluster = cg::this_cluster();
     const int blocks = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int64_t row = blockIdx.x / blocks, slice = per_warp * kWarps, v = a.v;
+    const int64_t slice = per_warp * kWarps, v = a.v;
     const int64_t s0 = min(rank * slice, v), size = min(slice, v - s0);
+    for (int64_t row = blockIdx.x / blocks; row < a.rows; row += gridDim.x / blocks) {
     const T* const x = (const T*)a.logits + row * v + s0;
     auto key_at = [&](int64_t i) -> Key { return RESIDENT ? (Key)keys[i] : O::key(x[i]); };
     const int64_t w0 = min(warp * per_warp, size), w1 = min(w0 + per_warp, size);
-    // f(key, valid) on this warp's values, all lanes of the warp together
-    auto each = [&](auto&& f) {
-        for (int64_t i = w0 + lane; i < w1; i += 32) f(key_at(i));
+    // f(key) for this warp's keys of at least `from`, which is 1 or more; in shared memory 16 bytes at a
+    // time, most of which have none once a border is known to be above
+    auto each = [&](Key from, auto&& f) {
+        if (RESIDENT) {
+            constexpr int W = 16 / sizeof(typename O::Stored);
+            const typename O::Stored* const at = keys + warp * per_warp;
+            for (int i = lane * W; i < (int)per_warp; i += 32 * W) {
+                const Pack<typename O::Stored, W> q = *(const Pack<typename O::Stored, W>*)(at + i);
+                if (!any_from(q, from)) continue;
+#pragma unroll
+                for (int j = 0; j < W; ++j)
+                    if (q.v[j] >= from) f((Key)q.v[j]);
+            }
+        } else {
+            for (int64_t i = w0 + lane; i < w1; i += 32) {
+                const Key k = key_at(i);
+                if (k >= from) f(k);
+            }
+        }
     };
 
     // the largest key
     Key top = 0;
     if (RESIDENT) {
-        for (int64_t i = (int64_t)tid * V; i < size; i += (int64_t)kThreads * V) {
-            if (V == 1 || i + V <= size) {
-                const Pack<T, V> p = *(const Pack<T, V>*)(x + i);
+        // what is left of the slice behind the row: 0, below every key
+        constexpr int kTogether = 4;       // loads on their way at once
+        for (int i0 = tid * V; i0 < (int)slice; i0 += kTogether * kThreads * V) {
+            Pack<T, V> p[kTogether];
+#pragma unroll
+            for (int m = 0; m < kTogether; ++m)
+                if (i0 + m * kThreads * V < size) p[m] = *(const Pack<T, V>*)(x + i0 + m * kThreads * V);
+#pragma unroll
+            for (int m = 0; m < kTogether; ++m) {
+                const int i = i0 + m * kThreads * V;
+                if (i >= (int)slice) break;
                 Pack<typename O::Stored, V> q;
 #pragma unroll
-                for (int j = 0; j < V; ++j) {
-                    const Key k = O::key(p.v[j]);
-                    top = k > top ? k : top;
-                    q.v[j] = (typename O::Stored)k;
-                }
+                for (int j = 0; j < V; ++j) q.v[j] = 0;
+                if (i < size) q = keys_of<T, V>(p[m]);
                 *(Pack<typename O::Stored, V>*)(keys + i) = q;
-            } else {
-                for (int64_t j = i; j < size; ++j) {
-                    const Key k = O::key(x[j]);
-                    top = k > top ? k : top;
-                    keys[j] = (typename O::Stored)k;
-                }
+#pragma unroll
+                for (int j = 0; j < V; ++j) top = q.v[j] > top ? q.v[j] : top;
             }
         }
     } else {
-        each([&](Key k) { top = k > top ? k : top; });
+        each(1, [&](Key k) { top = k > top ? k : top; });
     }
     for (int i = tid; i < 2 * kBins * M::kWords; i += kThreads) (&sh.bins[0][0])[i] = 0;
+    const Key own_top = top;
     top = warp_max(top);
     if (lane == 0) sh.top[warp] = top;
     __syncthreads();
@@ -257,77 +296,79 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(SampleArgs a, int64_t 
     const bool none = most == -INFINITY, greedy = !(temp > 0), alone = greedy || most == INFINITY;
     // differences are taken of halves, which do not overflow
     const A half = most * A(0.5), scale = greedy ? A(0) : A(2 * 1.4426950408889634) / temp;
-    auto weight = [&](Key k) -> A {
-        const A e = O::value(k);
-        return k == top ? A(1) : alone || e == -INFINITY ? A(0) : power((e * A(0.5) - half) * scale);
+    // log2 of a weight, negated; infinite where the weight is 0
+    auto depth = [&](Key k) -> A {
+        const A e = O::value(k), d = (half - e * A(0.5)) * scale;
+        return k == top ? A(0) : alone || e == -INFINITY ? (A)INFINITY : d;
     };
+    auto weight = [&](Key k) { return power(-depth(k)); };
     auto mass = [&](Key k) { return M::of(weight(k), shift); };
 
     // ---- borders ----
     // The key at which the sum over the kept values in descending order reaches a target, the sum above
     // it and its own: the number of values, or their weight.  `aim` gives the target for the sum of all.
     int turn = 0;
-    Key edge = greedy ? top : 0;       // keys above the edge are kept, and the first `ties` at it
+    Key edge = greedy ? top : 1;       // keys above the edge are kept, and the first `ties` at it
     u64 ties = greedy ? 1 : ~0ULL, tied = ~0ULL;
     struct Border { Key key; u64 above, own; };
-    auto border_of = [&](auto by_weight, auto&& aim) -> Border {
+    // first round: bins of equal steps in log2 e, the last one open
+    const A wide = A(2) / (scale * kBinsPerOctave);
+    auto bin_of = [&](A depth) { return (int)fmin(depth * A(kBinsPerOctave), A(kBins - 1)); };
+    auto octave_bin = [&](Key k) { return bin_of(depth(k)); };
+    // keys not below and not above any of a bin, however bin and value were rounded
+    auto slack_of = [&](int bin) { return (fabs(most) + (A)(bin + 1) * wide) * (sizeof(A) == 8 ? A(1e-14) : A(1e-6)); };
+    auto bin_high = [&](int bin) { return bin > 0 ? min(top, O::at_least(most - (A)bin * wide + slack_of(bin))) : top; };
+    auto bin_low = [&](int bin) { return bin < kBins - 1 ? max((Key)1, O::at_most(most - (A)(bin + 1) * wide - slack_of(bin))) : (Key)1; };
+    // Adds up all blocks' histograms of this turn; the bin in which the sum from the top reaches
+    // target(sum of all), or -1; sh.before and sh.own are the sums above it and of it.
+    auto search = [&](auto by_weight, u64 above, auto&& target_of) -> int {
         constexpr bool kWeight = decltype(by_weight)::value;
-        // first round: bins of equal steps in log2 e, the last one open
-        const A step = scale * kBinsPerOctave;
-        auto octave_bin = [&](Key k) -> int {
-            const A d = (half - O::value(k) * A(0.5)) * step;
-            return k == top ? 0 : d < kBins - 1 ? (int)d : kBins - 1;
-        };
+        cluster.sync();
+        unsigned* const bins = sh.bins[turn & 1];
+        const u64 own = M::template sum<!kWeight>(tid, blocks, [&](int q) { return cluster.map_shared_rank(bins, (rank + q) & (blocks - 1)); });
+        if (tid == 0) sh.found = -1;
+        u64 total;
+        const u64 before = above + block_prefix(own, sh.scan, &total);
+        const u64 target = target_of(total);
+        if (before < target && target <= before + own) {
+            sh.found = tid;
+            sh.before = before;
+            sh.own = own;
+        }
+        // the other histogram is free: all blocks have passed the barrier behind its last use
+        ++turn;
+        for (int i = tid; i < kBins * M::kWords; i += kThreads) sh.bins[turn & 1][i] = 0;
+        __syncthreads();
+        return sh.found;
+    };
+    auto border_of = [&](auto by_weight, Key floor, auto&& aim) -> Border {
+        constexpr bool kWeight = decltype(by_weight)::value;
         int octave = -1, down = 0;
-        Key high = top, low = 0;
+        Key high = top, low = max(floor, edge);
         u64 above = 0, target = 0;
-        // a round leaves 1/1024 of the span or less: 8 are the most for 64-bit keys
+        // a round leaves 1/256 of the span or less: 9 are the most for 64-bit keys
         for (int round = 0; round < 12; ++round) {
             unsigned* const bins = sh.bins[turn & 1];
-            each([&](Key k) {
-                if (k < edge || k < low || k > high) return;
-                int bin;
-                if (octave < 0) {
-                    bin = octave_bin(k);
-                } else {
-                    if (octave_bin(k) != octave) return;
+            each(low, [&](Key k) {
+                if (k > high) return;
+                const A d = depth(k);
+                int bin = bin_of(d);
+                if (octave >= 0) {
+                    if (bin != octave) return;
                     bin = (int)((high - k) >> down);
                 }
-                if (kWeight) M::add(bins, bin, weight(k), shift);
+                if (kWeight) M::add(bins, bin, power(-d), shift);
                 else M::count(bins, bin);
             });
-            cluster.sync();
-            u64 own[2] = {0, 0};
-            M::template sum<!kWeight>(own, tid, blocks, [&](int q) { return cluster.map_shared_rank(bins, (rank + q) & (blocks - 1)); });
-            if (tid == 0) sh.found = -1;
-            u64 total;
-            u64 before = above + block_prefix(own[0] + own[1], sh.scan, &total);
-            if (octave < 0) target = aim(total);
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                if (before < target && target <= before + own[i]) {
-                    sh.found = 2 * tid + i;
-                    sh.before = before;
-                    sh.own = own[i];
-                }
-                before += own[i];
-            }
-            // the other histogram is free: all blocks have passed the barrier behind its last use
-            ++turn;
-            for (int i = tid; i < kBins * M::kWords; i += kThreads) sh.bins[turn & 1][i] = 0;
-            __syncthreads();
-            const int found = sh.found;
+            const int found = search(by_weight, above, [&](u64 total) { return target = octave < 0 ? aim(total) : target; });
             if (found < 0) break;
             above = sh.before;
             const u64 mine = sh.own;
             __syncthreads();
             if (octave < 0) {
                 octave = found;
-                // a span that has all of the bin's keys, however the bin and the span were rounded;
-                // whether a key is in the bin is for octave_bin to say
-                const A wide = A(2) / step, slack = (fabs(most) + (A)(found + 1) * wide) * (sizeof(A) == 8 ? A(1e-14) : A(1e-6));
-                if (found > 0) high = min(top, O::at_least(most - (A)found * wide + slack));
-                if (found < kBins - 1) low = O::at_most(most - (A)(found + 1) * wide - slack);
+                high = bin_high(found);
+                low = max(low, bin_low(found));
             } else {
                 high -= (Key)found << down;
                 const Key span = ((Key)1 << down) - 1;
@@ -342,7 +383,16 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(SampleArgs a, int64_t 
     if (!greedy && !none) {
         const double kk = row_param(a.top_k, row);
         if (kk >= 1 && kk < (double)v) {
-            const Border b = border_of(std::false_type(), [&](u64) { return (u64)kk; });
+            // the k-th largest of all threads' own largest keys is not above the k-th largest key: with it
+            // the first histogram is of a few values instead of all
+            Key floor = 1;
+            if (kk <= (double)(blocks * kThreads)) {
+                if (own_top) M::count(sh.bins[turn & 1], octave_bin(own_top));
+                const int found = search(std::false_type(), 0, [&](u64) { return (u64)kk; });
+                if (found >= 0) floor = bin_low(found);
+                __syncthreads();
+            }
+            const Border b = border_of(std::false_type(), floor, [&](u64) { return (u64)kk; });
             edge = b.key;
             ties = (u64)kk - b.above;
             tied = b.own;
@@ -350,7 +400,7 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(SampleArgs a, int64_t 
         const double pp = row_param(a.top_p, row);
         if (pp < 1) {
             u64 need = 0;
-            const Border b = border_of(std::true_type(), [&](u64 sum) {
+            const Border b = border_of(std::true_type(), (Key)1, [&](u64 sum) {
                 if (ties < tied) sum -= (tied - ties) * mass(edge);
                 const double want = ceil(pp * (double)sum);
                 need = want >= 1 ? min((u64)want, sum) : 1;
@@ -366,9 +416,10 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(SampleArgs a, int64_t 
     const A least = (A)fmin(row_param(a.min_p, row), 1.0);   // the largest logit stays
     if (!(weight(edge) >= least)) ties = 0;
     u64 mine = 0, at_edge = 0;
-    each([&](Key k) {
-        if (k == edge) ++at_edge;
-        else if (k > edge) {
+    each(edge, [&](Key k) {
+        if (k == edge) {
+            ++at_edge;
+        } else {
             const A e = weight(k);
             if (e >= least) mine += M::of(e, shift);
         }
@@ -405,38 +456,43 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(SampleArgs a, int64_t 
         a.token[row] = -1;
         ((A*)a.logp)[row] = -INFINITY;
     }
-    if (warp == sh.found) {
-        u64 sum = sh.before, rank_of_tie = sh.extra;
-        for (int64_t i0 = w0; i0 < w1; i0 += 32) {
-            const int64_t i = i0 + lane;
-            const Key k = i < w1 ? key_at(i) : 0;
-            const unsigned equal = __ballot_sync(0xffffffffu, i < w1 && k == edge);
-            const bool tie = i < w1 && k == edge && rank_of_tie + __popc(equal & ((1u << lane) - 1)) < ties;
-            rank_of_tie += __popc(equal);
-            u64 s = 0;
-            if (tie || (i < w1 && k > edge && weight(k) >= least)) s = mass(k);
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const u64 w = __shfl_up_sync(0xffffffffu, s, o);
-                if (lane >= o) s += w;
+    const int owner = sh.found;
+    if (owner >= 0) {
+        // the draw lies in the values of one warp of this block: all threads look for it, each in a
+        // piece of neighbouring values
+        const u64 first = sh.before, first_tie = sh.extra;
+        const int64_t o0 = min(owner * per_warp, size), o1 = min(o0 + per_warp, size), piece = (per_warp + kThreads - 1) / kThreads;
+        const int64_t i0 = min(o0 + tid * piece, o1), i1 = min(i0 + piece, o1);
+        u64 equal = 0, sum = 0;
+        for (int64_t i = i0; i < i1; ++i) equal += key_at(i) == edge;
+        const u64 tie0 = first_tie + block_prefix(equal, sh.scan, &unused);
+        auto walk = [&](auto&& stop) {
+            u64 tie = tie0, s = 0;
+            for (int64_t i = i0; i < i1; ++i) {
+                const Key k = key_at(i);
+                if (k == edge ? tie++ >= ties : k < edge || !(weight(k) >= least)) continue;
+                s += mass(k);
+                if (stop(s, i, k)) break;
             }
-            const unsigned past = __ballot_sync(0xffffffffu, sum + s > aim);
-            if (past) {
-                if (lane == __ffs(past) - 1) {
-                    a.token[row] = (int)(s0 + i);
-                    const double e = k == top ? 0.0 : ((double)O::value(k) - (double)most) / (double)temp;
-                    ((A*)a.logp)[row] = (A)(e - log((double)total / (double)(1ULL << shift)));
-                }
-                break;
-            }
-            sum += __shfl_sync(0xffffffffu, s, 31);
-        }
+            return s;
+        };
+        sum = walk([](u64, int64_t, Key) { return false; });
+        const u64 here = first + block_prefix(sum, sh.scan, &unused);
+        if (here <= aim && aim < here + sum)
+            walk([&](u64 s, int64_t i, Key k) {
+                if (here + s <= aim) return false;
+                a.token[row] = (int)(s0 + i);
+                const double e = k == top ? 0.0 : ((double)O::value(k) - (double)most) / (double)temp;
+                ((A*)a.logp)[row] = (A)(e - log((double)total / (double)(1ULL << shift)));
+                return true;
+            });
     }
-    cluster.sync();    // no block's shared memory goes while another may read it
+    cluster.sync();    // no block's shared memory goes, or has the next row, while another may read it
+    }
 }
 
 template <typename T, int V, bool WIDE, bool RESIDENT>
-cudaError_t launch(const SampleArgs& a, int blocks, int64_t per_warp, int shift, cudaStream_t s) {
+cudaError_t launch(const SampleArgs& a, int blocks, int64_t per_warp, int shift, int sm_count, cudaStream_t s) {
     const size_t bytes = (sizeof(SampleShared<T, WIDE>) + 15) / 16 * 16 + (RESIDENT ? (size_t)per_warp * kWarps * sizeof(typename Order<T>::Stored) : 0);
     const auto kernel = sample_kernel<T, V, WIDE, RESIDENT>;
     if (bytes > 48 * 1024) {
@@ -444,7 +500,11 @@ cudaError_t launch(const SampleArgs& a, int blocks, int64_t per_warp, int shift,
         if (e != cudaSuccess) return e;
     }
     cudaLaunchConfig_t config = {};
-    config.gridDim = dim3((unsigned)(a.rows * blocks));
+    // Clusters that are resident at once, as far as registers and shared memory tell (a cluster starts
+    // slower than a row that follows another in it), each with as many rows as the others.
+    const int64_t each_sm = std::min<int64_t>(2, 227 * 1024 / (int64_t)(bytes + 1024));
+    const int64_t most = std::max<int64_t>(sm_count * each_sm * 15 / 16 / blocks, 1), turns = (a.rows + most - 1) / most;
+    config.gridDim = dim3((unsigned)((a.rows + turns - 1) / turns * blocks));
     config.blockDim = dim3(kThreads);
     config.dynamicSmemBytes = bytes;
     config.stream = s;
@@ -463,17 +523,17 @@ cudaError_t sample(const SampleArgs& a, int sm_count, cudaStream_t s) {
     // as few blocks as hold a row, but more for few rows: their passes are shorter
     int blocks = 1;
     while (blocks < kMostBlocks && (a.v > blocks * kSlice || (a.rows * blocks * 2 <= sm_count && a.v > blocks * 4096))) blocks *= 2;
-    const int64_t per_warp = ((a.v + blocks - 1) / blocks + kWarps * 32 - 1) / (kWarps * 32) * 32, slice = per_warp * kWarps;
+    const int64_t per_warp = ((a.v + blocks - 1) / blocks + kWarps * kGrain - 1) / (kWarps * kGrain) * kGrain, slice = per_warp * kWarps;
     int shift = 62;                                             // v terms of at most 2^shift stay below 2^62
     while ((1LL << (62 - shift)) < a.v) --shift;
     if (a.rows * blocks >= (1LL << 31)) return cudaErrorInvalidValue;
     constexpr int V = 16 / sizeof(T);
     if (kDouble) {
-        if (slice > kSlice) return launch<T, 1, true, false>(a, blocks, per_warp, shift, s);
-        return a.v % V == 0 ? launch<T, V, true, true>(a, blocks, per_warp, shift, s) : launch<T, 1, true, true>(a, blocks, per_warp, shift, s);
+        if (slice > kSlice) return launch<T, 1, true, false>(a, blocks, per_warp, shift, sm_count, s);
+        return a.v % V == 0 ? launch<T, V, true, true>(a, blocks, per_warp, shift, sm_count, s) : launch<T, 1, true, true>(a, blocks, per_warp, shift, sm_count, s);
     } else {
-        if (slice > kSlice) return launch<T, 1, true, false>(a, blocks, per_warp, shift, s);
-        return a.v % V == 0 ? launch<T, V, false, true>(a, blocks, per_warp, 45, s) : launch<T, 1, false, true>(a, blocks, per_warp, 45, s);
+        if (slice > kSlice) return launch<T, 1, true, false>(a, blocks, per_warp, shift, sm_count, s);
+        return a.v % V == 0 ? launch<T, V, false, true>(a, blocks, per_warp, 45, sm_count, s) : launch<T, 1, false, true>(a, blocks, per_warp, 45, sm_count, s);
     }
 }
 
