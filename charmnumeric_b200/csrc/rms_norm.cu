@@ -4,9 +4,10 @@
 //   h = x + residual,   r = 1 / sqrt(mean(h^2) + eps),   y = h r w
 //
 // In 8 bits a group of columns is held as codes q and one scale:  with v = h w and a = max |v|,
-//   q = rint(v (127 / a)),   scale = a r / 127,   value = q scale.
-// r cancels out of q, so the codes depend on no sum and no order.  a = 0: codes and scale 0; a
-// infinite or NaN: codes 0 and scale NaN, so that every value of the group is NaN.
+//   q = rint(v ((1 / a) 127)),   scale = a r / 127,   value = q scale.
+// r cancels out of q, so the codes depend on no sum and no order.  a = 0, or so small that 1 / a
+// overflows: codes and scale 0; a infinite or NaN: codes 0 and scale NaN, so that every value of the
+// group is NaN.
 #include <algorithm>
 #include <type_traits>
 
@@ -86,6 +87,17 @@ struct Row {
         return RESIDUAL ? v + widen(r[i].v[j]) : v;
     }
 };
+
+// the factor from values to codes; 0 where the codes are
+template <typename A>
+__device__ __forceinline__ A code_factor(A most) {
+    const A f = A(1) / most * A(127);
+    return most > 0 && most < (A)INFINITY && f < (A)INFINITY ? f : A(0);
+}
+template <typename A>
+__device__ __forceinline__ A scale_of(A most, A factor, A r) {
+    return !(most < (A)INFINITY) ? (A)NAN : factor > 0 ? most * r / A(127) : A(0);
+}
 
 template <typename A>
 __device__ __forceinline__ A root(A squares, const RmsNormArgs& a) {
@@ -189,8 +201,7 @@ __global__ void __launch_bounds__(W == 1 ? 128 : W * 32) rms_norm_8_kernel(RmsNo
 #pragma unroll
     for (int i = 0; i < R; ++i) {
         if (!in.any(i)) break;
-        const bool fine = most[i] < (A)INFINITY;
-        const A f = fine && most[i] > 0 ? A(127) / most[i] : A(0);
+        const A f = code_factor(most[i]);
         Pack<T, V> h;
         Pack<signed char, V> q;
         A w[V];
@@ -199,12 +210,12 @@ __global__ void __launch_bounds__(W == 1 ? 128 : W * 32) rms_norm_8_kernel(RmsNo
         for (int j = 0; j < V; ++j) {
             const A v = in.sum(i, j);
             h.v[j] = narrow<T>(v);
-            q.v[j] = fine ? (signed char)(int)rint(v * w[j] * f) : (signed char)0;
+            q.v[j] = f > 0 ? (signed char)(int)rint(v * w[j] * f) : (signed char)0;
         }
         in.put(q, (signed char*)a.y, i);
         if (RESIDUAL) in.put(h, (T*)a.h, i);
         if (G == 0 ? tid == 0 && i == 0 : tid % (G ? G : 1) == 0)
-            ((A*)a.scale)[row * groups + (G == 0 ? 0 : in.at(i) / (int)a.group)] = fine ? most[i] * r / A(127) : (A)NAN;
+            ((A*)a.scale)[row * groups + (G == 0 ? 0 : in.at(i) / (int)a.group)] = scale_of(most[i], f, r);
     }
 }
 
@@ -251,15 +262,14 @@ __global__ void __launch_bounds__(256) rms_norm_long_kernel(RmsNormArgs a) {
             most = v <= most ? most : v == v ? v : (A)INFINITY;
         }
         most = warp_max(most);
-        const bool fine = most < (A)INFINITY;
-        const A f = most > 0 && fine ? A(127) / most : A(0);
+        const A f = code_factor(most);
         for (int64_t i = i0 + lane; i < i1; i += 32) {
             A h = widen(x[i]);
             if (res) h += widen(res[i]);
             const A v = w ? h * widen(w[i]) : h;
-            ((signed char*)a.y)[row * a.n + i] = fine ? (signed char)(int)rint(v * f) : (signed char)0;
+            ((signed char*)a.y)[row * a.n + i] = f > 0 ? (signed char)(int)rint(v * f) : (signed char)0;
         }
-        if (lane == 0) ((A*)a.scale)[row * groups + g] = fine ? most * r / A(127) : (A)NAN;
+        if (lane == 0) ((A*)a.scale)[row * groups + g] = scale_of(most, f, r);
     }
 }
 

@@ -59,8 +59,10 @@ def rms_norm(x, weight=None, *, residual=None, eps=1e-6, bits=None, group=None):
 
     Returns ``y``, or ``(y, h)`` with a residual.  With ``bits=8`` the result is held as int8 codes and
     one scale for every ``group`` columns (default: the whole row): ``(codes, scale)``, or
-    ``(codes, scale, h)``; ``dequantize`` gives the values.  A group that is all zero has codes and
-    scale 0, one with an infinity or a NaN codes 0 and scale NaN.
+    ``(codes, scale, h)``; ``dequantize`` gives the values.  With ``v = h * weight`` and a group's largest
+    ``|v|``, a, codes are ``rint(v * (1 / a * 127))``, whatever the row's norm.  A group that is all zero (or
+    so small that 1 / a overflows) has codes and scale 0, one with an infinity or a NaN codes 0 and
+    scale NaN.
     """
     x = _activations(x, "x", (1, 2, 3))
     n = x.shape[-1]

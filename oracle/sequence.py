@@ -40,9 +40,10 @@ def rms_norm(x, weight, residual, eps, group, to=None):
                 part = v[..., i:i + g]
                 most = np.abs(part).max(-1, keepdims=True)
                 fine = np.isfinite(most)
-                factor = np.where(fine & (most > 0), acc(127) / most, acc(0)).astype(acc)
-                codes[..., i:i + g] = np.where(fine, np.rint(part * factor), 0).astype(np.int8)
-                scales.append(np.where(fine, _wide(most) * r / 127.0, np.nan))
+                factor = (acc(1) / most * acc(127)).astype(acc)
+                factor = np.where(fine & (most > 0) & np.isfinite(factor), factor, acc(0))
+                codes[..., i:i + g] = np.where(factor > 0, np.rint(part * factor), 0).astype(np.int8)
+                scales.append(np.where(fine, np.where(factor > 0, _wide(most) * r / 127.0, 0.0), np.nan))
             results = [codes, np.concatenate(scales, -1).astype(acc)]
     return results + ([h.astype(x.dtype)] if _given(residual) else [])
 
