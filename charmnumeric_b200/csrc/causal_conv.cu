@@ -39,10 +39,25 @@ __global__ void __launch_bounds__(kThreads) causal_conv_kernel(CausalConvArgs a,
     const int64_t c = id % across * V, t0 = id / across * run, t1 = min(t0 + run, a.t);
     const int pad = K - a.k;
     A w[K][V], bias[V];
+    if constexpr (V * sizeof(T) == 16 && K < kMaxConvWidth) {
+        // the filters of V channels are K pieces of 16 bytes
+        T f[K * V];
 #pragma unroll
-    for (int j = 0; j < K; ++j)
+        for (int i = 0; i < K; ++i) {
+            const Pack<T, V> p = *(const Pack<T, V>*)((const T*)a.weight + c * K + i * V);
 #pragma unroll
-        for (int v = 0; v < V; ++v) w[j][v] = j >= pad ? widen(((const T*)a.weight)[(c + v) * a.k + j - pad]) : A(0);
+            for (int v = 0; v < V; ++v) f[i * V + v] = p.v[v];
+        }
+#pragma unroll
+        for (int j = 0; j < K; ++j)
+#pragma unroll
+            for (int v = 0; v < V; ++v) w[j][v] = widen(f[v * K + j]);
+    } else {
+#pragma unroll
+        for (int j = 0; j < K; ++j)
+#pragma unroll
+            for (int v = 0; v < V; ++v) w[j][v] = j >= pad ? widen(((const T*)a.weight)[(c + v) * a.k + j - pad]) : A(0);
+    }
 #pragma unroll
     for (int v = 0; v < V; ++v) bias[v] = a.bias ? widen(((const T*)a.bias)[c + v]) : A(0);
     Pack<T, V> zero;

@@ -145,9 +145,27 @@ __global__ void __launch_bounds__(W == 1 ? 128 : W * 32) rms_norm_kernel(RmsNorm
     }
 }
 
+// The larger of a value (of at least 0, or NaN) and |v|, where NaN is the largest: as integers the bits are
+// in that order.
+__device__ __forceinline__ float most_of(float most, float v) {
+    return __uint_as_float(max(__float_as_uint(most), __float_as_uint(v) & 0x7fffffffu));
+}
+__device__ __forceinline__ double most_of(double most, double v) {
+    return __longlong_as_double(max(__double_as_longlong(most), __double_as_longlong(v) & 0x7fffffffffffffffLL));
+}
+
+// v f, rounded to the nearest whole number of -127 to 127.  Added to 1.5 2^23 (2^52) the number is in the
+// last bits; no product may go into that sum.
+__device__ __forceinline__ signed char code_of(float v, float f) {
+    return (signed char)__float_as_uint(__fadd_rn(__fmul_rn(v, f), 12582912.0f));
+}
+__device__ __forceinline__ signed char code_of(double v, double f) {
+    return (signed char)__double_as_longlong(__dadd_rn(__dmul_rn(v, f), 6755399441055744.0));
+}
+
 // The same with the 8-bit output.  The lanes that share a group of columns find its largest value
 // together: G lanes for groups of G pieces (a power of two up to a warp), or the whole block for one
-// scale a row (G = 0).
+// scale a row (G = 0).  h is stored, and h w kept, before the row's sum is known.
 template <typename T, int V, int R, int W, int G, bool RESIDUAL, bool WHOLE>
 __global__ void __launch_bounds__(W == 1 ? 128 : W * 32) rms_norm_8_kernel(RmsNormArgs a) {
     using A = typename Acc<T>::type;
@@ -156,43 +174,41 @@ __global__ void __launch_bounds__(W == 1 ? 128 : W * 32) rms_norm_8_kernel(RmsNo
     if (row >= a.rows) return;
     Row<T, V, R, W, RESIDUAL, WHOLE> in;
     in.load(a, row, tid);
-    A s = 0, most[R];
-    // a NaN counts as infinity: it makes the group's scale NaN like one
+    A s = 0, most[R], v[R][V];
 #pragma unroll
     for (int i = 0; i < R; ++i) {
         most[i] = 0;
         if (in.any(i)) {
             A w[V];
+            Pack<T, V> h;
             in.weight(w, a, i);
 #pragma unroll
             for (int j = 0; j < V; ++j) {
-                const A h = in.sum(i, j), v = fabs(h * w[j]);
+                const A x = in.sum(i, j);
+                h.v[j] = narrow<T>(x);
+                v[i][j] = x * w[j];
                 if (!in.has(i, j)) continue;
-                s += h * h;
-                most[i] = v <= most[i] ? most[i] : v == v ? v : (A)INFINITY;
+                s += x * x;
+                most[i] = most_of(most[i], v[i][j]);
             }
+            if (RESIDUAL) in.put(h, (T*)a.h, i);
         }
     }
     __shared__ A sm[W], sm_most[W];
     if (G == 0) {
 #pragma unroll
-        for (int i = 1; i < R; ++i) most[0] = most[i] > most[0] ? most[i] : most[0];
-        most[0] = warp_max(most[0]);
-        if (W > 1 && (tid & 31) == 0) sm_most[tid >> 5] = most[0];
-    } else {
-#pragma unroll
-        for (int i = 0; i < R; ++i)
-#pragma unroll
-            for (int o = G / 2; o > 0; o >>= 1) {
-                const A v = __shfl_xor_sync(0xffffffffu, most[i], o);
-                most[i] = v > most[i] ? v : most[i];
-            }
+        for (int i = 1; i < R; ++i) most[0] = most_of(most[0], most[i]);
     }
+#pragma unroll
+    for (int i = 0; i < (G == 0 ? 1 : R); ++i)
+#pragma unroll
+        for (int o = (G == 0 ? 16 : G / 2); o > 0; o >>= 1) most[i] = most_of(most[i], __shfl_xor_sync(0xffffffffu, most[i], o));
+    if (G == 0 && W > 1 && (tid & 31) == 0) sm_most[tid >> 5] = most[0];
     s = W == 1 ? warp_sum(s) : block_sum(s, sm);    // its barrier covers sm_most
     if (G == 0) {
         if (W > 1)
 #pragma unroll
-            for (int i = 0; i < W; ++i) most[0] = sm_most[i] > most[0] ? sm_most[i] : most[0];
+            for (int i = 0; i < W; ++i) most[0] = most_of(most[0], sm_most[i]);
 #pragma unroll
         for (int i = 1; i < R; ++i) most[i] = most[0];
     }
@@ -202,18 +218,10 @@ __global__ void __launch_bounds__(W == 1 ? 128 : W * 32) rms_norm_8_kernel(RmsNo
     for (int i = 0; i < R; ++i) {
         if (!in.any(i)) break;
         const A f = code_factor(most[i]);
-        Pack<T, V> h;
         Pack<signed char, V> q;
-        A w[V];
-        in.weight(w, a, i);
 #pragma unroll
-        for (int j = 0; j < V; ++j) {
-            const A v = in.sum(i, j);
-            h.v[j] = narrow<T>(v);
-            q.v[j] = f > 0 ? (signed char)(int)rint(v * w[j] * f) : (signed char)0;
-        }
+        for (int j = 0; j < V; ++j) q.v[j] = f > 0 ? code_of(v[i][j], f) : (signed char)0;
         in.put(q, (signed char*)a.y, i);
-        if (RESIDUAL) in.put(h, (T*)a.h, i);
         if (G == 0 ? tid == 0 && i == 0 : tid % (G ? G : 1) == 0)
             ((A*)a.scale)[row * groups + (G == 0 ? 0 : in.at(i) / (int)a.group)] = scale_of(most[i], f, r);
     }
@@ -258,16 +266,16 @@ __global__ void __launch_bounds__(256) rms_norm_long_kernel(RmsNormArgs a) {
                 h += widen(res[i]);
                 ((T*)a.h)[row * a.n + i] = narrow<T>(h);
             }
-            const A v = fabs(w ? h * widen(w[i]) : h);
-            most = v <= most ? most : v == v ? v : (A)INFINITY;
+            most = most_of(most, w ? h * widen(w[i]) : h);
         }
-        most = warp_max(most);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) most = most_of(most, __shfl_xor_sync(0xffffffffu, most, o));
         const A f = code_factor(most);
         for (int64_t i = i0 + lane; i < i1; i += 32) {
             A h = widen(x[i]);
             if (res) h += widen(res[i]);
             const A v = w ? h * widen(w[i]) : h;
-            ((signed char*)a.y)[row * a.n + i] = f > 0 ? (signed char)(int)rint(v * f) : (signed char)0;
+            ((signed char*)a.y)[row * a.n + i] = f > 0 ? code_of(v, f) : (signed char)0;
         }
         if (lane == 0) ((A*)a.scale)[row * groups + g] = scale_of(most, f, r);
     }
@@ -297,7 +305,8 @@ cudaError_t launch_long(const RmsNormArgs& a, cudaStream_t s) {
     return cudaGetLastError();
 }
 
-// One warp for up to 4 pieces a thread, else as few warps as hold the row in 4 pieces a thread.
+// One warp for up to 4 pieces a thread, else as few warps (4 to 32) as hold the row in 4, in 3 where that
+// does: threads without a piece cost (1531 rows of 5003 floats: 28.0 us in 4 by 16 warps, 24.8 in 3).
 template <typename T, bool WHOLE>
 cudaError_t by_length(const RmsNormArgs& a, cudaStream_t s) {
     constexpr int V = 16 / sizeof(T);
@@ -305,8 +314,11 @@ cudaError_t by_length(const RmsNormArgs& a, cudaStream_t s) {
     if (pieces <= 32) return launch_row<T, V, 1, 1, WHOLE>(a, s);
     if (pieces <= 128) return launch_row<T, V, 4, 1, WHOLE>(a, s);
     if (pieces <= 256) return launch_row<T, V, 2, 4, WHOLE>(a, s);
+    if (pieces <= 384) return launch_row<T, V, 3, 4, WHOLE>(a, s);
     if (pieces <= 512) return launch_row<T, V, 4, 4, WHOLE>(a, s);
+    if (pieces <= 768) return launch_row<T, V, 3, 8, WHOLE>(a, s);
     if (pieces <= 1024) return launch_row<T, V, 4, 8, WHOLE>(a, s);
+    if (pieces <= 1536) return launch_row<T, V, 3, 16, WHOLE>(a, s);
     if (pieces <= 2048) return launch_row<T, V, 4, 16, WHOLE>(a, s);
     if (pieces <= 4096) return launch_row<T, V, 4, 32, WHOLE>(a, s);
     return launch_long<T>(a, s);
@@ -373,22 +385,38 @@ __global__ void __launch_bounds__(256) convert_kernel(const From* in, To* out, i
     }
 }
 
-// Values of codes: V neighbouring codes of a row and group a thread, rows down blockIdx.y; bound by HBM.
+// Values of codes: V neighbouring codes of a row and group a thread, rows down blockIdx.y, four of them on
+// their way at once; bound by HBM.
 template <typename To, typename S, int V>
 __global__ void __launch_bounds__(256)
 dequantize_kernel(const signed char* in, const S* scale, To* out, int64_t rows, int64_t n, int64_t group, int64_t groups) {
+    constexpr int kRows = 4, kWide = 16 / sizeof(To) < V ? 16 / sizeof(To) : V;
     const int64_t col = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) * V;
     if (col >= n) return;
-    const int64_t g = col / group;
-    for (int64_t row = (int64_t)blockIdx.y * blockDim.y + threadIdx.y; row < rows; row += (int64_t)gridDim.y * blockDim.y) {
-        const Pack<signed char, V> q = *(const Pack<signed char, V>*)(in + row * n + col);
-        const S f = scale[row * groups + g];
-        alignas(16) To v[V];
+    const int64_t g = col / group, down = (int64_t)gridDim.y * blockDim.y;
+    for (int64_t row0 = (int64_t)blockIdx.y * blockDim.y + threadIdx.y; row0 < rows; row0 += kRows * down) {
+        Pack<signed char, V> q[kRows];
+        S f[kRows];
 #pragma unroll
-        for (int j = 0; j < V; ++j) v[j] = narrow<To>((typename Acc<To>::type)((S)q.v[j] * f));
-        constexpr int W = 16 / sizeof(To) < V ? 16 / sizeof(To) : V;
+        for (int k = 0; k < kRows; ++k) {
+            const int64_t row = row0 + k * down;
+            if (row < rows) {
+                q[k] = *(const Pack<signed char, V>*)(in + row * n + col);
+                f[k] = scale[row * groups + g];
+            }
+        }
 #pragma unroll
-        for (int j = 0; j < V; j += W) *(Pack<To, W>*)(out + row * n + col + j) = *(Pack<To, W>*)&v[j];
+        for (int k = 0; k < kRows; ++k) {
+            const int64_t row = row0 + k * down;
+            if (row >= rows) break;
+#pragma unroll
+            for (int j = 0; j < V; j += kWide) {
+                Pack<To, kWide> v;
+#pragma unroll
+                for (int m = 0; m < kWide; ++m) v.v[m] = narrow<To>((typename Acc<To>::type)((S)q[k].v[j + m] * f[k]));
+                *(Pack<To, kWide>*)(out + row * n + col + j) = v;
+            }
+        }
     }
 }
 
@@ -428,7 +456,9 @@ cudaError_t dequantize(const ConvertArgs& a, int sm_count, cudaStream_t s) {
 template <typename To, typename S>
 cudaError_t dequantize(const ConvertArgs& a, int sm_count, cudaStream_t s) {
     const bool whole = a.group >= a.n;
-    if (a.n % 8 == 0 && (whole || a.group % 8 == 0)) return dequantize<To, S, 8>(a, sm_count, s);
+    // as many codes as make one 16-byte store
+    constexpr int V = 16 / sizeof(To);
+    if (a.n % V == 0 && (whole || a.group % V == 0)) return dequantize<To, S, V>(a, sm_count, s);
     return dequantize<To, S, 1>(a, sm_count, s);
 }
 
