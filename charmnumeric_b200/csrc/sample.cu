@@ -13,11 +13,13 @@
 // the first two filters come down to one border in the order of the logits, (key, number of ties kept).
 // NaN counts as -infinity.  A row with +infinities draws among them alone.
 //
-// Nothing is sorted.  A cluster of up to 8 blocks has a row, each block a slice of it in shared memory as
+// A cluster of up to 8 blocks has a row, each block a slice of it in shared memory as
 // integer keys in the order of the values, read from HBM once.  A border is found by histograms: the
 // first over steps of 1/16 in log2 e, the next over what the bin with the border spans in key space,
 // 512 times finer each time, until a bin is one key.  Every block adds up all blocks' histograms
-// (distributed shared memory), so that one cluster barrier a round is enough.
+// (distributed shared memory), so that one cluster barrier a round is enough.  A top-k of a few hundred
+// leaves few values above a bound that is found from each thread's largest key; those are brought
+// together and ordered by counting, and the rest of the work is on that list.
 #include <cooperative_groups.h>
 
 #include <algorithm>
@@ -36,7 +38,7 @@ namespace {
 typedef unsigned long long u64;
 
 constexpr int kThreads = 512, kWarps = kThreads / 32, kBins = kThreads, kMostBlocks = 8;
-constexpr int kBinsPerOctave = 16, kGrain = 256;
+constexpr int kBinsPerOctave = 16, kGrain = 256, kList = kThreads;
 
 // Integers in the order of the values; -0 and 0 are one value, NaN the lowest.
 template <typename T> struct Order;
@@ -185,6 +187,11 @@ struct SampleShared {
     typename Order<T>::Key top[kWarps], most;
     u64 before, own, extra, total;                             // what a search has found
     int found;
+    // a short list of the largest values, of this block and then (in the first block) of the row
+    int listed;
+    typename Order<T>::Key list_key[kList], row_key[kList];
+    int list_at[kList], row_at[kList];
+    u64 row_mass[kList];
 };
 
 // exclusive prefix sum over the block, in the order of the threads
@@ -380,6 +387,59 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 8 ? 1 : 2) sample_kerne
         }
         return {edge, above, 0};    // not reached: a target is never above the sum of all
     };
+    // Writes down the token that `aim_of(total)` and the sums of kept weights decide on.
+    const double u = a.u_dtype == DT_F64 ? ((const double*)a.u)[row] : (double)((const float*)a.u)[row];
+    auto aim_of = [&](u64 total) {
+        const u64 aim = u > 0 ? (u >= 1 ? total : (u64)(u * (double)total)) : 0;
+        return aim >= total ? total - 1 : aim;
+    };
+    auto write = [&](Key k, int at, u64 total) {
+        a.token[row] = at;
+        const double e = k == top ? 0.0 : ((double)O::value(k) - (double)most) / (double)temp;
+        ((A*)a.logp)[row] = (A)(e - log((double)total / (double)(1ULL << shift)));
+    };
+    const A least = (A)fmin(row_param(a.min_p, row), 1.0);   // the largest logit stays
+    // The first block draws from the `count` largest values of the row, one a thread: the first `k` in
+    // their order, then top-p, min-p and the draw as everywhere.
+    auto draw_from = [&](int count, int from, int place, int k) {
+        Key key = 0;
+        int at = 0;
+        if (tid < count) {
+            key = cluster.map_shared_rank(sh.list_key, from)[place];
+            at = cluster.map_shared_rank(sh.list_at, from)[place];
+            sh.row_key[tid] = key;
+            sh.row_at[tid] = at;
+        }
+        __syncthreads();
+        int order = 0;
+        for (int i = 0; i < count; ++i) order += sh.row_key[i] > key || (sh.row_key[i] == key && sh.row_at[i] < at);
+        __syncthreads();
+        if (tid < count) {
+            sh.row_key[order] = key;
+            sh.row_at[order] = at;
+        }
+        __syncthreads();
+        const int kept_k = min(k, count);
+        key = tid < kept_k ? sh.row_key[tid] : 0;
+        at = sh.row_at[tid < kept_k ? tid : 0];
+        u64 m = tid < kept_k ? mass(key) : 0, sum, total;
+        const u64 before = block_prefix(m, sh.scan, &sum);
+        const double pp = row_param(a.top_p, row);
+        if (pp < 1) {
+            const double want = ceil(pp * (double)sum);
+            const u64 need = want >= 1 ? min((u64)want, sum) : 1;
+            if (before >= need) m = 0;
+        }
+        if (tid < kept_k && !(weight(key) >= least)) m = 0;
+        sh.row_mass[tid] = m;
+        block_prefix(m, sh.scan, &total);
+        __syncthreads();
+        u64 upto = 0;
+        for (int i = 0; i < kept_k; ++i) upto += sh.row_at[i] <= at ? sh.row_mass[i] : 0;
+        const u64 aim = aim_of(total);
+        if (m && upto - m <= aim && aim < upto) write(key, at, total);
+    };
+    bool short_list = false;
     if (!greedy && !none) {
         const double kk = row_param(a.top_k, row);
         if (kk >= 1 && kk < (double)v) {
@@ -388,17 +448,50 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 8 ? 1 : 2) sample_kerne
             Key floor = 1;
             if (kk <= (double)(blocks * kThreads)) {
                 if (own_top) M::count(sh.bins[turn & 1], octave_bin(own_top));
+                if (tid == 0) sh.listed = 0;
                 const int found = search(std::false_type(), 0, [&](u64) { return (u64)kk; });
                 if (found >= 0) floor = bin_low(found);
                 __syncthreads();
+                if (RESIDENT && kk <= kList / 2 && found >= 0) {
+                    constexpr int W = 16 / sizeof(typename O::Stored);
+                    for (int i = tid * W; i < (int)slice; i += kThreads * W) {
+                        const Pack<typename O::Stored, W> q = *(const Pack<typename O::Stored, W>*)(keys + i);
+                        if (!any_from(q, floor)) continue;
+#pragma unroll
+                        for (int j = 0; j < W; ++j) {
+                            if (q.v[j] < floor) continue;
+                            const int place = atomicAdd(&sh.listed, 1);
+                            if (place < kList) {
+                                sh.list_key[place] = q.v[j];
+                                sh.list_at[place] = (int)s0 + i + j;
+                            }
+                        }
+                    }
+                    cluster.sync();
+                    int count = 0, from = 0, place = tid;
+                    for (int q = 0; q < blocks; ++q) {
+                        const int theirs = *cluster.map_shared_rank(&sh.listed, q);
+                        if (count <= tid && tid < count + theirs) {
+                            from = q;
+                            place = tid - count;
+                        }
+                        count += theirs;
+                    }
+                    if (count <= kList) {     // the same in all blocks
+                        if (rank == 0) draw_from(count, from, place, (int)kk);
+                        short_list = true;
+                    }
+                }
             }
+            if (!short_list) {
             const Border b = border_of(std::false_type(), floor, [&](u64) { return (u64)kk; });
             edge = b.key;
             ties = (u64)kk - b.above;
             tied = b.own;
+            }
         }
         const double pp = row_param(a.top_p, row);
-        if (pp < 1) {
+        if (pp < 1 && !short_list) {
             u64 need = 0;
             const Border b = border_of(std::true_type(), (Key)1, [&](u64 sum) {
                 if (ties < tied) sum -= (tied - ties) * mass(edge);
@@ -413,7 +506,7 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 8 ? 1 : 2) sample_kerne
     }
 
     // ---- the draw ----
-    const A least = (A)fmin(row_param(a.min_p, row), 1.0);   // the largest logit stays
+    if (!short_list) {
     if (!(weight(edge) >= least)) ties = 0;
     u64 mine = 0, at_edge = 0;
     each(edge, [&](Key k) {
@@ -441,9 +534,7 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 8 ? 1 : 2) sample_kerne
     const u64 tied_before = block_prefix(count, sh.scan, &unused);
     if (ties > tied_before) theirs += min(count, ties - tied_before) * mass(edge);
     const u64 before = block_prefix(theirs, sh.scan, &total);
-    const double u = a.u_dtype == DT_F64 ? ((const double*)a.u)[row] : (double)((const float*)a.u)[row];
-    u64 aim = u > 0 ? (u >= 1 ? total : (u64)(u * (double)total)) : 0;
-    if (aim >= total) aim = total - 1;
+    const u64 aim = aim_of(total);
     if (tid == 0) sh.found = -1;
     __syncthreads();
     if (!none && before <= aim && aim < before + theirs && tid / kWarps == rank) {
@@ -481,11 +572,10 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 8 ? 1 : 2) sample_kerne
         if (here <= aim && aim < here + sum)
             walk([&](u64 s, int64_t i, Key k) {
                 if (here + s <= aim) return false;
-                a.token[row] = (int)(s0 + i);
-                const double e = k == top ? 0.0 : ((double)O::value(k) - (double)most) / (double)temp;
-                ((A*)a.logp)[row] = (A)(e - log((double)total / (double)(1ULL << shift)));
+                write(k, (int)(s0 + i), total);
                 return true;
             });
+    }
     }
     cluster.sync();    // no block's shared memory goes, or has the next row, while another may read it
     }
