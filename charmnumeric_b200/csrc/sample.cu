@@ -371,7 +371,7 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 8 ? 1 : 2) sample_kerne
             if (found < 0) break;
             above = sh.before;
             const u64 mine = sh.own;
-            __syncthreads();
+            // the next search writes these behind barriers that every thread passes after this
             if (octave < 0) {
                 octave = found;
                 high = bin_high(found);
@@ -382,8 +382,8 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 8 ? 1 : 2) sample_kerne
                 low = high - low > span ? high - span : low;
             }
             if (low == high) return {high, above, mine};
-            down = 0;
-            while (((high - low) >> down) >= (Key)kBins) ++down;
+            const int bits = 64 - __clzll((u64)(high - low));    // of the span; bins of it have 9
+            down = bits > 9 ? bits - 9 : 0;
         }
         return {edge, above, 0};    // not reached: a target is never above the sum of all
     };
@@ -451,7 +451,6 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 8 ? 1 : 2) sample_kerne
                 if (tid == 0) sh.listed = 0;
                 const int found = search(std::false_type(), 0, [&](u64) { return (u64)kk; });
                 if (found >= 0) floor = bin_low(found);
-                __syncthreads();
                 if (RESIDENT && kk <= kList / 2 && found >= 0) {
                     constexpr int W = 16 / sizeof(typename O::Stored);
                     for (int i = tid * W; i < (int)slice; i += kThreads * W) {
