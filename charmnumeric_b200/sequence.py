@@ -120,11 +120,13 @@ def _sequences(x, lengths):
     return _operand(lengths, "lengths", (_I32,), (x.shape[0],))
 
 
-def _state_result(state, inplace, shape, dtype):
+def _state_result(given, state, inplace, others, shape, dtype):
     if not inplace:
         return _new_array(shape, dtype)
-    if state is None:
-        raise ValueError("inplace needs a state")
+    if state is None or state is not given:
+        raise ValueError("inplace needs the state as a whole array")
+    if any(o is not None and o._info is state._info for o in others):
+        raise ValueError("a state that is updated in place cannot be another operand too")
     return state
 
 
@@ -150,13 +152,11 @@ def causal_conv(x, weight, bias=None, *, state=None, lengths=None, activation=No
     bias = _operand(bias, "bias", (x.dtype,), (d,))
     given = state
     state = _operand(state, "state", (x.dtype,), (b, k - 1, d))
-    if inplace and state is not given:
-        raise ValueError("inplace needs the state as a whole array")
     lengths = _sequences(x, lengths)
     if activation not in (None, "silu"):
         raise ValueError(f'activation must be None or "silu", got {activation!r}')
+    after = _state_result(given, state, inplace, (x, weight, bias, lengths), (b, k - 1, d), x.dtype)
     y = _new_array(x.shape, x.dtype)
-    after = _state_result(state, inplace, (b, k - 1, d), x.dtype)
     _apply(wire.OP_CAUSAL_CONV, [x, weight, bias, state, lengths, 1 if activation else 0], [y, after])
     return y, after
 
@@ -195,11 +195,9 @@ def selective_scan(x, delta, A, B, C, *, D=None, z=None, delta_bias=None, softpl
     delta_bias = _operand(delta_bias, "delta_bias", (acc,), (d,))
     given = state
     state = _operand(state, "state", (acc,), (b, d, n))
-    if inplace and state is not given:
-        raise ValueError("inplace needs the state as a whole array")
     lengths = _sequences(x, lengths)
+    after = _state_result(given, state, inplace, (x, delta, A, B, C, D, z, delta_bias, lengths), (b, d, n), acc)
     y = _new_array(x.shape, x.dtype)
-    after = _state_result(state, inplace, (b, d, n), acc)
     _apply(wire.OP_SELECTIVE_SCAN, [x, delta, A, B, C, D, z, delta_bias, state, lengths, 1 if softplus else 0], [y, after])
     return y, after
 

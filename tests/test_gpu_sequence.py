@@ -640,3 +640,136 @@ def test_a_model_step(interface):
     gpu, cpu = run_both(interface, program)
     for k in cpu:
         np.testing.assert_allclose(gpu[k], cpu[k], rtol=1e-9, atol=1e-12, err_msg=k)
+
+
+# ---- what the backend itself refuses -------------------------------------------------------------------------------
+
+def _leaf(ctx, name, array):
+    from charmnumeric_b200 import wire
+    from charmnumeric_b200.context import WIRE_DTYPES
+    ctx.put(name, array)
+    return wire.leaf(name, array.shape, WIRE_DTYPES[array.dtype])
+
+
+def _cases():
+    from charmnumeric_b200 import wire
+    f = np.float32
+    none = wire.scalar(0.0)
+    x2, x3 = np.ones((3, 8), f), np.ones((2, 5, 4), f)
+    scan = [x3, x3, -np.ones((4, 3), f), np.ones((2, 5, 3), f), np.ones((2, 5, 3), f), none, none, none, none, none, wire.scalar(1)]
+    def put(i, v, base):
+        return base[:i] + [v] + base[i + 1:]
+    norm, conv = [x2, none, none, wire.scalar(1e-5), wire.scalar(0)], [x3, np.ones((4, 3), f), none, none, none, wire.scalar(0)]
+    draw = [x2, np.ones(3, f), wire.scalar(1), wire.scalar(0), wire.scalar(1), wire.scalar(0)]
+    return [
+        (wire.OP_RMS_NORM, put(0, x2.astype("int32"), norm), 1, 7), (wire.OP_RMS_NORM, put(1, np.ones(7, f), norm), 1, 4),
+        (wire.OP_RMS_NORM, put(2, np.ones((3, 9), f), norm), 2, 4), (wire.OP_RMS_NORM, put(2, x2.astype("float16"), norm), 2, 7),
+        (wire.OP_RMS_NORM, put(3, wire.scalar(float("nan")), norm), 1, 1), (wire.OP_RMS_NORM, put(4, wire.scalar(9), norm), 2, 1),
+        (wire.OP_RMS_NORM, put(4, wire.scalar(1.5), norm), 2, 1), (wire.OP_RMS_NORM, norm, 2, 2), (wire.OP_RMS_NORM, norm[:4], 1, 2),
+        (wire.OP_RMS_NORM, put(0, none, norm), 1, 2),
+        (wire.OP_CAUSAL_CONV, put(0, x2, conv), 2, 4), (wire.OP_CAUSAL_CONV, put(1, np.ones((5, 3), f), conv), 2, 4),
+        (wire.OP_CAUSAL_CONV, put(1, np.ones((4, 9), f), conv), 2, 5), (wire.OP_CAUSAL_CONV, put(3, np.ones((2, 3, 4), f), conv), 2, 4),
+        (wire.OP_CAUSAL_CONV, put(4, np.ones(2, f), conv), 2, 7), (wire.OP_CAUSAL_CONV, put(4, np.ones(3, "int32"), conv), 2, 4),
+        (wire.OP_CAUSAL_CONV, put(5, wire.scalar(2), conv), 2, 1), (wire.OP_CAUSAL_CONV, conv, 1, 2),
+        (wire.OP_SELECTIVE_SCAN, put(1, x3[:1], scan), 2, 4), (wire.OP_SELECTIVE_SCAN, put(2, -np.ones((4, 257), f), scan), 2, 5),
+        (wire.OP_SELECTIVE_SCAN, put(2, -np.ones((4, 3)), scan), 2, 7), (wire.OP_SELECTIVE_SCAN, put(3, np.ones((2, 5, 4), f), scan), 2, 4),
+        (wire.OP_SELECTIVE_SCAN, put(4, np.ones((2, 5, 6), f), scan), 2, 4), (wire.OP_SELECTIVE_SCAN, put(8, np.ones((2, 4, 2), f), scan), 2, 4),
+        (wire.OP_SELECTIVE_SCAN, put(7, np.ones(5, f), scan), 2, 4), (wire.OP_SELECTIVE_SCAN, scan[:10], 2, 2),
+        (wire.OP_SAMPLE, put(1, np.ones(2, f), draw), 2, 4), (wire.OP_SAMPLE, put(1, np.ones(3, "int32"), draw), 2, 7),
+        (wire.OP_SAMPLE, put(3, np.ones(3, f), draw), 2, 7), (wire.OP_SAMPLE, put(4, np.ones(4, f), draw), 2, 4),
+        (wire.OP_SAMPLE, put(0, x3, draw), 2, 4), (wire.OP_SAMPLE, draw, 1, 2),
+        (wire.OP_CONVERT, [x2, np.ones((3, 1), f), wire.scalar(8)], 1, 7),
+        (wire.OP_CONVERT, [x2.astype("int8"), np.ones((3, 2), f), wire.scalar(8)], 1, 4),
+        (wire.OP_CONVERT, [x2.astype("int8"), np.ones((3, 1), f), wire.scalar(0)], 1, 1),
+        (99, [x2], 1, 6),
+    ]
+
+
+@pytest.mark.parametrize("case", range(36))
+def test_backend_refusals(interface, case):
+    from charmnumeric_b200 import wire
+    from charmnumeric_b200._lib import CnError
+    ctx = interface.context
+    opcode, operands, results, status = _cases()[case]
+    leaves = [(_leaf(ctx, 880100 + i, v) if isinstance(v, np.ndarray) else v, None) for i, v in enumerate(operands)]
+    roots = [wire.Ast(880200, opcode, shape=(1,), dtype=wire.F32, operands=leaves)]
+    roots += [wire.Ast(880200 + i, wire.OP_NOOP, shape=(1,), dtype=wire.F32) for i in range(1, results)]
+    before = ctx.stats()["kernel_launches"]
+    with pytest.raises(CnError) as e:
+        ctx.run([wire.Node(0, roots, fusible=False)])
+    assert e.value.status == status, e.value
+    assert ctx.stats()["kernel_launches"] == before
+    ctx.synchronize()                                  # the context stays usable
+    for i, v in enumerate(operands):
+        if isinstance(v, np.ndarray):
+            ctx.delete_array(880100 + i)
+
+
+def test_backend_refuses_results_that_are_operands(interface):
+    from charmnumeric_b200 import wire
+    from charmnumeric_b200._lib import CnError
+    ctx = interface.context
+    x = _leaf(ctx, 880300, np.ones((2, 1, 4), np.float32))
+    w = _leaf(ctx, 880301, np.ones((4, 2), np.float32))
+    none, noop = wire.scalar(0.0), lambda n: wire.Ast(n, wire.OP_NOOP, shape=(1,), dtype=wire.F32)  # noqa: E731
+    def conv(y, state, operand=none):
+        return [wire.Ast(y, wire.OP_CAUSAL_CONV, shape=(1,), dtype=wire.F32, operands=[(v, None) for v in (x, w, none, operand, none, none)]), noop(state)]
+    for roots in (conv(880300, 880310), conv(880310, 880301), conv(880310, 880310), conv(880310, 880300, x)):
+        with pytest.raises(CnError) as e:
+            ctx.run([wire.Node(0, roots, fusible=False)])
+        assert e.value.status == 11
+    np.testing.assert_array_equal(ctx.get(880300), 1)
+    for name in (880300, 880301):
+        ctx.delete_array(name)
+
+
+def test_host_memory_is_no_device_array(interface):
+    from charmnumeric_b200._lib import CnError
+    host = np.zeros(16, np.float32)
+    class Fake:
+        __cuda_array_interface__ = {"shape": (16,), "typestr": "<f4", "data": (host.ctypes.data, False), "version": 3}
+    with pytest.raises(CnError) as e:
+        cnp.from_device(interface, Fake())
+    assert e.value.status == 1
+
+
+def test_two_contexts_at_once(interface):
+    """Two interfaces on one GPU, each with its own arrays and stream, interleaved."""
+    rng = np.random.default_rng(3)
+    other = cnp.CharmNumericInterface(device=0)
+    try:
+        x = [rng.standard_normal((40, 30000)).astype("float32") for _ in range(2)]
+        u = rng.random(40).astype("float32")
+        steps = []
+        for itf, v in zip((interface, other), x):
+            a, b = cnp.asarray(v), cnp.asarray(u)
+            cnp.execute(itf)
+            steps.append((itf, cnp.record(lambda: cnp.random.sample(a, b, top_k=30, top_p=0.9))))
+        for _ in range(20):
+            for itf, step in steps:
+                step.run(itf)
+        for (itf, step), v in zip(steps, x):
+            check_samples(v, step.results[0].get(itf), step.results[1].get(itf), u, 1.0, 30, 0.9, 0.0)
+    finally:
+        del steps
+        other.close()
+
+
+def test_a_long_decoding_loop_in_place(interface):
+    """A recorded step that brings its states up to date itself, against the prompt's scan."""
+    rng = np.random.default_rng(31)
+    b, t, d, n = 4, 24, 64, 16
+    a = scan_inputs(rng, b, t, d, n, "float32")
+    x, delta, B, C, zz = (cnp.zeros((b, 1, v.shape[2]), dtype="float32") for v in (a["x"], a["delta"], a["B"], a["C"], a["z"]))
+    state = cnp.asarray(a["state"])
+    fixed = {k: cnp.asarray(a[k]) for k in ("A", "D", "delta_bias")}
+    cnp.execute(interface)
+    step = cnp.record(lambda: cnp.selective_scan(x, delta, fixed["A"], B, C, D=fixed["D"], z=zz, delta_bias=fixed["delta_bias"], state=state, inplace=True))
+    ys = []
+    for i in range(t):
+        for to, k in ((x, "x"), (delta, "delta"), (B, "B"), (C, "C"), (zz, "z")):
+            interface.context.put(to.name, np.ascontiguousarray(a[k][:, i:i + 1]))
+        ys.append(step.run(interface)[0].get(interface))
+    y, yo, h, ho = scan_exact(a)
+    check(np.concatenate(ys, 1), y, yo, "float32")
+    check(state.get(interface), h, ho, "float32")

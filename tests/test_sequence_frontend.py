@@ -168,3 +168,32 @@ def test_storage_arrays_never_join_a_fused_group():
         kinds = {r.dtype for r in n.roots}
         assert len(kinds) == 1, kinds
     assert c.dtype == np.float32
+
+
+def test_a_state_in_place_is_no_other_operand():
+    s = z(2, 1, 4)
+    with pytest.raises(ValueError):
+        cnp.causal_conv(s, z(4, 2), state=s, inplace=True)
+    w = z(2, 4, 4)
+    with pytest.raises(ValueError):
+        cnp.selective_scan(w, z(2, 4, 4), z(4, 4), z(2, 4, 4), z(2, 4, 4), state=w, inplace=True)
+
+
+def test_a_recorded_step_keeps_what_it_uses():
+    """Arrays of a step are released when both the program and the step have let go of them."""
+    import gc
+    x = z(3, 4)
+    F._state.pending, F._state.dead = [], []
+    x._info.materialised = True
+    step = cnp.record(lambda: cnp.rms_norm(x))
+    names = {x.name, step.results.name}
+    del x
+    gc.collect()
+    assert not names & set(F._state.dead)
+    step.results = None
+    gc.collect()
+    assert not names & set(F._state.dead)
+    del step
+    gc.collect()
+    assert names <= set(F._state.dead)
+    F._state.dead = []
