@@ -773,3 +773,13 @@ def test_a_long_decoding_loop_in_place(interface):
     y, yo, h, ho = scan_exact(a)
     check(np.concatenate(ys, 1), y, yo, "float32")
     check(state.get(interface), h, ho, "float32")
+
+
+@pytest.mark.parametrize("t", [1, 50])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_selective_scan_steps_of_no_size_change_nothing(interface, t, dtype):
+    rng = np.random.default_rng(17)
+    a = scan_inputs(rng, 5, t, 256, 16, dtype)
+    a["delta"][...] = -1200.0 if dtype == "float64" else -300.0     # softplus is exactly 0
+    gpu, _ = run_both(interface, lambda: dict(zip("ys", run_scan(a))))
+    bits(gpu["s"], a["state"])
