@@ -9,6 +9,7 @@ import hashlib
 import os
 import subprocess
 import sys
+from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
 HERE = Path(__file__).resolve().parent
@@ -20,7 +21,7 @@ ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 HOST_SOURCES = ["wire.cpp", "lower.cpp", "fuse.cpp", "regions.cpp", "decomp.cpp", "codegen.cpp", "jit.cpp", "comm.cpp", "context.cpp",
                 "executor.cpp", "sequence.cpp", "capi.cpp"]
 SEQUENCE_SOURCES = ["rms_norm.cu", "causal_conv.cu", "selective_scan.cu", "sample.cu"]
-CUDA_SOURCES = ["kernels.cu", "noalloc.cu"] + SEQUENCE_SOURCES
+CUDA_SOURCES = ["kernels.cu", "noalloc.cu", "storage.cu"] + SEQUENCE_SOURCES
 
 
 def _embed():
@@ -68,25 +69,30 @@ def build(force=False, verbose=False):
     emb = _embed()
     common = ["-O3", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC,-Wall,-Wno-unused-function",
               "-I", str(CSRC), "-I", str(BUILD)]
-    objs = []
-    for src in [CSRC / s for s in HOST_SOURCES] + [emb]:
+    def compile_one(src):
         obj = BUILD / (src.stem + ".o")
-        cmd = [NVCC, "-x", "cu"] + ARCH + common + ["-c", str(src), "-o", str(obj)]
+        if src.suffix == ".cu":
+            cmd = [NVCC] + ARCH + common + ["-Xptxas", "-v", "-c", str(src), "-o", str(obj)]
+        else:
+            cmd = [NVCC, "-x", "cu"] + ARCH + common + ["-c", str(src), "-o", str(obj)]
         if verbose:
             print(" ".join(cmd))
-        subprocess.run(cmd, check=True)
-        objs.append(obj)
-    for s in cuda_sources:
-        src = CSRC / s
-        obj = BUILD / (src.stem + ".o")
-        cmd = [NVCC] + ARCH + common + ["-Xptxas", "-v", "-c", str(src), "-o", str(obj)]
-        if verbose:
-            print(" ".join(cmd))
-        res = subprocess.run(cmd, check=True, capture_output=True, text=True)
-        (BUILD / (src.stem + ".ptxas.txt")).write_text(res.stderr)
-        if verbose:
+        res = subprocess.run(cmd, capture_output=True, text=True)
+        if res.returncode:
+            sys.stderr.write(res.stdout + res.stderr)
+            res.check_returncode()
+        if src.suffix == ".cu":
+            (BUILD / (src.stem + ".ptxas.txt")).write_text(res.stderr)
+        elif res.stderr:
+            sys.stderr.write(res.stderr)
+        if verbose and src.suffix == ".cu":
             print(res.stderr)
-        objs.append(obj)
+        return obj
+
+    # the longest first: selective_scan.cu alone takes as long as all host sources together
+    sources = [CSRC / s for s in reversed(cuda_sources)] + [CSRC / s for s in HOST_SOURCES] + [emb]
+    with ThreadPoolExecutor(max_workers=max(1, min(8, os.cpu_count() or 1))) as pool:
+        objs = list(pool.map(compile_one, sources))
     cmd = [NVCC, "-shared"] + ARCH + ["-o", str(OUT)] + [str(o) for o in objs] + ["-ldl", "-lpthread"]
     if verbose:
         print(" ".join(cmd))

@@ -8,6 +8,7 @@
 #include <vector>
 
 #include "kernels.hpp"
+#include "storage.hpp"
 #include "regions.hpp"
 
 namespace cn {
@@ -1018,7 +1019,7 @@ int Context::try_plain_fill(const DagNode& node, bool* done) {
             if (d > 0) v.off += reg.start[d] * strides[d];
         }
         if (n0 > 0 && ext[1] > 0 && ext[2] > 0 && ext[0] > 0) {
-            rc = cuda_fail(launch_fill_region(a->buf.data, a->dtype, v, ext, r->operands[1].leaf->scalar, stream_), "fill");
+            rc = cuda_fail((dtype_valid(a->dtype) ? launch_fill_region : launch_storage_fill)(a->buf.data, a->dtype, v, ext, r->operands[1].leaf->scalar, stream_), "fill");
             if (rc) return rc;
             stats_.kernel_launches++;
         }

@@ -10,6 +10,7 @@
 
 #include "context.hpp"
 #include "kernels.hpp"
+#include "storage.hpp"
 #include "regions.hpp"
 
 namespace cn {
@@ -1314,7 +1315,7 @@ int Context::execute_cross_set_region(const AstNode& r) {
         }
         // the target's dimension 0 starts at position i0: advance the source along the dimension it maps to
         if (map[0] >= 0) sv.off += i0 * sreg.step[map[0]] * ss[map[0]];
-        rc = cuda_fail(launch_copy_region(t->buf.data, dv, sdata, sv, ext, t->dtype, stream_), "cross-dimension copy");
+        rc = cuda_fail((dtype_valid(t->dtype) ? launch_copy_region : launch_storage_copy)(t->buf.data, dv, sdata, sv, ext, t->dtype, stream_), "cross-dimension copy");
         if (rc) return rc;
         stats_.kernel_launches++;
     }
@@ -1400,7 +1401,7 @@ int Context::execute_diag(const AstNode& r) {
         return fail(CN_ERR_UNSUPPORTED, "DIAG needs a 1-D or 2-D array");
     }
     if (ext[2] > 0) {
-        rc = cuda_fail(launch_copy_region(out->buf.data, dv, sdata, sv, ext, dtype, stream_), "diag");
+        rc = cuda_fail((dtype_valid(dtype) ? launch_copy_region : launch_storage_copy)(out->buf.data, dv, sdata, sv, ext, dtype, stream_), "diag");
         if (rc) return rc;
         stats_.kernel_launches++;
     }
@@ -1460,7 +1461,7 @@ int Context::execute_tile(const AstNode& r) {
         if ((rc = group.end())) return rc;
         src = scratch_;
     }
-    rc = cuda_fail(launch_tile(out->buf.data, oshape, out->row_begin, out->local_rows(), src, sshape, dtype, stream_), "tile");
+    rc = cuda_fail((dtype_valid(dtype) ? launch_tile : launch_storage_tile)(out->buf.data, oshape, out->row_begin, out->local_rows(), src, sshape, dtype, stream_), "tile");
     if (rc) return rc;
     stats_.kernel_launches++;
     out->mark_written();

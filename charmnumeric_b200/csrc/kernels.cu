@@ -2,8 +2,6 @@
 // sum with the deterministic two-pass finish, and the row-block matrix-vector product.
 // All of them are bandwidth-bound; none uses tensor cores (no path here is a dense
 // contraction with reuse).
-#include <cuda_fp16.h>
-
 #include <algorithm>
 
 #include "cn_device.cuh"
@@ -252,8 +250,6 @@ cudaError_t launch_fill_region(void* base, int dtype, const StridedView& v, cons
         case DT_F32: fill_region_kernel<float><<<grid, 256, 0, s>>>((float*)base, vw, (float)value, n); break;
         case DT_F64: fill_region_kernel<double><<<grid, 256, 0, s>>>((double*)base, vw, value, n); break;
         case DT_I32: fill_region_kernel<int><<<grid, 256, 0, s>>>((int*)base, vw, (int)value, n); break;
-        case DT_F16: fill_region_kernel<__half><<<grid, 256, 0, s>>>((__half*)base, vw, __double2half(value), n); break;
-        case DT_I8: fill_region_kernel<signed char><<<grid, 256, 0, s>>>((signed char*)base, vw, (signed char)value, n); break;
         default: fill_region_kernel<long long><<<grid, 256, 0, s>>>((long long*)base, vw, (long long)value, n); break;
     }
     return cudaGetLastError();
@@ -268,10 +264,6 @@ cudaError_t launch_copy_region(void* dst, const StridedView& dv, const void* src
     int grid = grid_for(n, 256);
     if (dtype_size(dtype) == 8)
         copy_region_kernel<long long><<<grid, 256, 0, s>>>((long long*)dst, d, (const long long*)src, sr, n);
-    else if (dtype_size(dtype) == 2)
-        copy_region_kernel<short><<<grid, 256, 0, s>>>((short*)dst, d, (const short*)src, sr, n);
-    else if (dtype_size(dtype) == 1)
-        copy_region_kernel<signed char><<<grid, 256, 0, s>>>((signed char*)dst, d, (const signed char*)src, sr, n);
     else
         copy_region_kernel<int><<<grid, 256, 0, s>>>((int*)dst, d, (const int*)src, sr, n);
     return cudaGetLastError();
@@ -370,12 +362,6 @@ cudaError_t launch_tile(void* dst, const int64_t dst_shape[3], int64_t dst_row_b
     if (dtype_size(dtype) == 8)
         tile_kernel<long long><<<grid, 256, 0, s>>>((long long*)dst, dst_shape[1], dst_shape[2], dst_row_begin, n,
                                                     (const long long*)src, src_shape[0], src_shape[1], src_shape[2]);
-    else if (dtype_size(dtype) == 2)
-        tile_kernel<short><<<grid, 256, 0, s>>>((short*)dst, dst_shape[1], dst_shape[2], dst_row_begin, n,
-                                                (const short*)src, src_shape[0], src_shape[1], src_shape[2]);
-    else if (dtype_size(dtype) == 1)
-        tile_kernel<signed char><<<grid, 256, 0, s>>>((signed char*)dst, dst_shape[1], dst_shape[2], dst_row_begin, n,
-                                                      (const signed char*)src, src_shape[0], src_shape[1], src_shape[2]);
     else
         tile_kernel<int><<<grid, 256, 0, s>>>((int*)dst, dst_shape[1], dst_shape[2], dst_row_begin, n,
                                               (const int*)src, src_shape[0], src_shape[1], src_shape[2]);

@@ -1,0 +1,96 @@
+// Fills, strided copies and tiles of arrays of the storage types (float16, int8), which have no
+// arithmetic: a value is moved by its size.  Bound by HBM where the innermost dimension is dense;
+// these are set-up paths, and one value a thread and turn is what the other types' copies do too.
+#include <cuda_fp16.h>
+
+#include <algorithm>
+
+#include "cn_types.hpp"
+#include "kernels.hpp"
+#include "storage.hpp"
+
+namespace cn {
+
+namespace {
+
+constexpr int kThreads = 256;
+
+// element strides of up to three dimensions, and the extents they are walked over
+struct Walk {
+    int64_t ext[3], off, str[3];
+    __device__ __forceinline__ int64_t at(int64_t i) const {
+        const int64_t i2 = i % ext[2], t = i / ext[2];
+        return off + t / ext[1] * str[0] + t % ext[1] * str[1] + i2 * str[2];
+    }
+};
+
+template <typename T>
+__global__ void __launch_bounds__(kThreads) fill_kernel(T* to, Walk w, T value, int64_t n) {
+    for (int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x; i < n; i += (int64_t)gridDim.x * kThreads) to[w.at(i)] = value;
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kThreads) copy_kernel(T* to, Walk w, const T* from, Walk r, int64_t n) {
+    for (int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x; i < n; i += (int64_t)gridDim.x * kThreads) to[w.at(i)] = from[r.at(i)];
+}
+
+// w.off: the first row of the result; r.ext: the shape that is repeated
+template <typename T>
+__global__ void __launch_bounds__(kThreads) repeat_kernel(T* to, Walk w, const T* from, Walk r, int64_t n) {
+    for (int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x; i < n; i += (int64_t)gridDim.x * kThreads) {
+        const int64_t i2 = i % w.ext[2], t = i / w.ext[2], i1 = t % w.ext[1], i0 = w.off + t / w.ext[1];
+        to[i] = from[(i0 % r.ext[0] * r.ext[1] + i1 % r.ext[1]) * r.ext[2] + i2 % r.ext[2]];
+    }
+}
+
+Walk walk(const StridedView& v, const int64_t ext[3]) {
+    Walk w;
+    w.off = v.off;
+    for (int d = 0; d < 3; ++d) {
+        w.str[d] = v.str[d];
+        w.ext[d] = std::max<int64_t>(ext[d], 1);
+    }
+    return w;
+}
+
+unsigned blocks_for(int64_t n) { return (unsigned)std::min<int64_t>((n + kThreads - 1) / kThreads, 148 * 16); }
+
+}  // namespace
+
+cudaError_t launch_storage_fill(void* base, int dtype, const StridedView& v, const int64_t ext[3], double value, cudaStream_t s) {
+    if (ext[0] <= 0) return cudaSuccess;
+    const Walk w = walk(v, ext);
+    const int64_t n = w.ext[0] * w.ext[1] * w.ext[2];
+    if (dtype == DT_F16) fill_kernel<<<blocks_for(n), kThreads, 0, s>>>((__half*)base, w, __double2half(value), n);
+    else if (dtype == DT_I8) fill_kernel<<<blocks_for(n), kThreads, 0, s>>>((signed char*)base, w, (signed char)(int)value, n);
+    else return cudaErrorInvalidValue;
+    return cudaGetLastError();
+}
+
+cudaError_t launch_storage_copy(void* dst, const StridedView& dv, const void* src, const StridedView& sv, const int64_t ext[3], int dtype, cudaStream_t s) {
+    if (ext[0] <= 0) return cudaSuccess;
+    const Walk w = walk(dv, ext), r = walk(sv, ext);
+    const int64_t n = w.ext[0] * w.ext[1] * w.ext[2];
+    if (dtype == DT_F16) copy_kernel<<<blocks_for(n), kThreads, 0, s>>>((short*)dst, w, (const short*)src, r, n);
+    else if (dtype == DT_I8) copy_kernel<<<blocks_for(n), kThreads, 0, s>>>((signed char*)dst, w, (const signed char*)src, r, n);
+    else return cudaErrorInvalidValue;
+    return cudaGetLastError();
+}
+
+cudaError_t launch_storage_tile(void* dst, const int64_t dst_shape[3], int64_t dst_row_begin, int64_t dst_rows, const void* src,
+                                const int64_t src_shape[3], int dtype, cudaStream_t s) {
+    const int64_t n = dst_rows * dst_shape[1] * dst_shape[2];
+    if (n <= 0) return cudaSuccess;
+    Walk w = {}, r = {};
+    w.off = dst_row_begin;
+    for (int d = 0; d < 3; ++d) {
+        w.ext[d] = dst_shape[d];
+        r.ext[d] = src_shape[d];
+    }
+    if (dtype == DT_F16) repeat_kernel<<<blocks_for(n), kThreads, 0, s>>>((short*)dst, w, (const short*)src, r, n);
+    else if (dtype == DT_I8) repeat_kernel<<<blocks_for(n), kThreads, 0, s>>>((signed char*)dst, w, (const signed char*)src, r, n);
+    else return cudaErrorInvalidValue;
+    return cudaGetLastError();
+}
+
+}  // namespace cn
