@@ -7,7 +7,8 @@ from .frontend import _new_array, _normalize_dtype, _normalize_shape, execute
 class DeviceView:
     """This rank's rows of an array where they are, for a library that reads
     ``__cuda_array_interface__``.  The interface names the stream the values are made on; a library
-    that does not order itself behind it has to (``stream`` is its handle)."""
+    that does not order itself behind it has to (``stream`` is its handle).  It shows the memory that the
+    array has now: a stencil sweep, or a prompt with its state in place, moves an array to other memory."""
 
     def __init__(self, array, shape, pointer, stream):
         self.array = array  # keeps it from being released

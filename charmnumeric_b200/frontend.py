@@ -159,6 +159,7 @@ class _State:
         self.pending = []
         self.next_node = 0
         self.auto_flush = None    # (interface, threshold)
+        self.recording = False    # inside of record(): what is pending is not to be executed
         # Names keep counting up across resets and the list of dead arrays is kept: arrays of
         # an earlier program may still live in a backend context and be released later, and a
         # late release must never hit a new array that happens to reuse the name.
@@ -1083,6 +1084,8 @@ def execute(interface, mirror=None):
     ``mirror`` (optional) is an object with ``run(nodes, deletes)`` and ``put(name, host)``
     that receives exactly what the backend receives, in the same order; the tests pass the
     CPU oracle here so both sides execute one and the same DAG."""
+    if _state.recording:
+        raise RuntimeError("a step that is being recorded cannot execute or fetch anything")
     ops, _state.pending = _state.pending, []
     ctx = getattr(interface, "context", None)
     if mirror is None:

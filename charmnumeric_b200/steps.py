@@ -37,14 +37,16 @@ class Step:
 
 
 def record(fn):
-    """The operations that ``fn()`` records, as a ``Step``.  It must not upload host data or fetch results."""
+    """The operations that ``fn()`` records, as a ``Step``.  It must not upload host data,
+    and nothing can be executed or fetched inside."""
     outer, F._state.pending = F._state.pending, []
     flush, F._state.auto_flush = F._state.auto_flush, None
+    within, F._state.recording = F._state.recording, True
     try:
         results = fn()
         ops = F._state.pending
     finally:
-        F._state.pending, F._state.auto_flush = outer, flush
+        F._state.pending, F._state.auto_flush, F._state.recording = outer, flush, within
     if any(op.kind == "put" for op in ops):
         raise ValueError("a recorded step uploads host data: make its arrays before")
     infos = {}

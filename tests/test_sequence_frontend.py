@@ -197,3 +197,31 @@ def test_a_recorded_step_keeps_what_it_uses():
     gc.collect()
     assert names <= set(F._state.dead)
     F._state.dead = []
+
+
+def test_a_step_executes_nothing_while_it_is_recorded():
+    class Nowhere:
+        context = None
+    F._state.pending = []
+    x = z(3, 4)
+    with pytest.raises(RuntimeError):
+        cnp.record(lambda: cnp.execute(Nowhere()))
+    with pytest.raises(RuntimeError):
+        cnp.record(lambda: cnp.rms_norm(x).get(Nowhere()))
+    assert not F._state.recording and len(F._state.pending) == 1    # x is still to be made
+    inner = []
+    outer = cnp.record(lambda: (inner.append(cnp.record(lambda: cnp.rms_norm(x))), cnp.rms_norm(x))[1])
+    assert outer.results.name != inner[0].results.name and not F._state.recording
+    F._state.pending, F._state.dead = [], []
+
+
+def test_the_profiled_kernels_built_ahead_of_time_are_the_ones_in_the_tree():
+    """A DRAM traffic capture counts for the source that it was taken from only."""
+    import hashlib
+    import json
+    from pathlib import Path
+    root = Path(__file__).resolve().parent.parent
+    csrc = root / "charmnumeric_b200" / "csrc"
+    now = hashlib.sha256((csrc / "kernels.cu").read_bytes() + (csrc / "kernels.hpp").read_bytes()).hexdigest()[:8]
+    entries = json.loads((root / "profiles" / "dram_traffic.json").read_text())["kernels"]
+    assert [e["code"] for e in entries if "matvec" in e["match"]] == ["#" + now]
