@@ -185,7 +185,7 @@ struct SampleShared {
     u64 weight[kWarps];                                        // each warp's kept weight above the border
     u64 tied[kWarps];                                          // ... and values at the border
     typename Order<T>::Key top[kWarps], most;
-    u64 before, own, extra, total;                             // what a search has found
+    u64 before, own, extra;                                    // what a search has found
     int found;
     // a short list of the largest values, of this block and then (in the first block) of the row
     int listed;
@@ -300,9 +300,11 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 8 ? 1 : 2) sample_kerne
     top = warp_max(top);
     const A most = O::value(top);
     const A temp = (A)row_param(a.temperature, row);
-    const bool none = most == -INFINITY, greedy = !(temp > 0), alone = greedy || most == INFINITY;
+    const bool none = most == -INFINITY, greedy = !(temp > 0);
     // differences are taken of halves, which do not overflow
     const A half = most * A(0.5), scale = greedy ? A(0) : A(2 * 1.4426950408889634) / temp;
+    // only the largest has weight: it is infinite, or the temperature so small that its inverse is
+    const bool alone = greedy || most == INFINITY || scale == INFINITY;
     // log2 of a weight, negated; infinite where the weight is 0
     auto depth = [&](Key k) -> A {
         const A e = O::value(k), d = (half - e * A(0.5)) * scale;

@@ -783,3 +783,41 @@ def test_selective_scan_steps_of_no_size_change_nothing(interface, t, dtype):
     a["delta"][...] = -1200.0 if dtype == "float64" else -300.0     # softplus is exactly 0
     gpu, _ = run_both(interface, lambda: dict(zip("ys", run_scan(a))))
     bits(gpu["s"], a["state"])
+
+
+@pytest.mark.parametrize("dtype", ["float16", "int8"])
+def test_storage_types_in_three_dimensions(interface, dtype):
+    """Steps in every dimension, diagonals and repeats."""
+    rng = np.random.default_rng(18)
+    x = (rng.standard_normal((7, 9, 11)) * 20).astype(dtype)
+    def program():
+        a = cnp.asarray(x)
+        part = a[1::2, ::3, 2:10:2].copy()
+        b = cnp.zeros((9, 10, 13), dtype=dtype)
+        b[2:9:3, 1:10:3, 5:9] = part
+        b[::4, 9, :] = 7
+        return {"part": part, "b": b, "tile": cnp.tile(a, (2, 1, 3)), "diag": cnp.diag(cnp.asarray(x[0]))}
+    gpu, cpu = run_both(interface, program)
+    for k in cpu:
+        bits(gpu[k], cpu[k])
+    bits(gpu["part"], np.ascontiguousarray(x[1::2, ::3, 2:10:2]))
+    bits(gpu["tile"], np.tile(x, (2, 1, 3)))
+    bits(gpu["diag"], np.diag(x[0]).copy())
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_sample_temperatures_without_an_inverse(interface, dtype):
+    """So small that 1 / temperature is infinite (in 32 bits): the largest logit, as at 0.  Neighbours of the
+    largest whose difference from it is next to nothing have no weight either."""
+    x = np.random.default_rng(22).standard_normal((3, 5000)).astype(dtype)
+    x[1] *= np.asarray(1e-3, dtype)
+    x[2] = np.where(np.arange(5000) % 2, x[2], 4).astype(dtype)       # 2500 equal ones: the draw is among them
+    u = np.array([0.2, 0.5, 0.9], "float32")
+    def program():
+        ax, au, out = cnp.asarray(x), cnp.asarray(u), {}
+        for i, (k, p) in enumerate([(0, 1.0), (50, 1.0), (0, 0.9), (4000, 0.5)]):
+            out[f"t{i}"], out[f"p{i}"] = cnp.random.sample(ax, au, temperature=1e-42, top_k=k, top_p=p)
+        return out
+    gpu, _ = run_both(interface, program)
+    for i, (k, p) in enumerate([(0, 1.0), (50, 1.0), (0, 0.9), (4000, 0.5)]):
+        check_samples(x, gpu[f"t{i}"], gpu[f"p{i}"], u, 1e-42, k, p, 0.0)
