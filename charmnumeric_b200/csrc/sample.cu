@@ -13,6 +13,8 @@
 // the first two filters come down to one border in the order of the logits, (key, number of ties kept).
 // NaN counts as -infinity.  A row with +infinities draws among them alone.
 //
+// Bound by latency: the bytes (a row's logits, once) are a tenth of the time or less, the rest are rounds of
+// a pass over shared memory, a cluster barrier and a prefix sum, one after the other.  So:
 // A cluster of up to 8 blocks has a row, each block a slice of it in shared memory as
 // integer keys in the order of the values, read from HBM once.  A border is found by histograms: the
 // first over steps of 1/16 in log2 e, the next over what the bin with the border spans in key space,
@@ -20,6 +22,12 @@
 // (distributed shared memory), so that one cluster barrier a round is enough.  A top-k of a few hundred
 // leaves few values above a bound that is found from each thread's largest key; those are brought
 // together and ordered by counting, and the rest of the work is on that list.
+//
+// 128 rows of 131072 in 16 bits, top-k 50, top-p 0.9, min-p 0.02: a block a row without shared memory 1592 us;
+// clusters with keys in shared memory 226; histograms read in wide, coalesced pieces 136; rows looped over
+// by resident clusters (a cluster starts slower than a row that follows another in it) 96; the short list
+// 54 us.  One row of 32768 with top-p alone: 419, 102, 27, 27, 24 us.
+// 1024 threads, and passes without branches, were slower.
 #include <cooperative_groups.h>
 
 #include <algorithm>
@@ -235,350 +243,350 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 8 ? 1 : 2) sample_kerne
     const int64_t slice = per_warp * kWarps, v = a.v;
     const int64_t s0 = min(rank * slice, v), size = min(slice, v - s0);
     for (int64_t row = blockIdx.x / blocks; row < a.rows; row += gridDim.x / blocks) {
-    const T* const x = (const T*)a.logits + row * v + s0;
-    auto key_at = [&](int64_t i) -> Key { return RESIDENT ? (Key)keys[i] : O::key(x[i]); };
-    const int64_t w0 = min(warp * per_warp, size), w1 = min(w0 + per_warp, size);
-    // f(key) for this warp's keys of at least `from`, which is 1 or more; in shared memory 16 bytes at a
-    // time, most of which have none once a border is known to be above
-    auto each = [&](Key from, auto&& f) {
-        if (RESIDENT) {
-            constexpr int W = 16 / sizeof(typename O::Stored);
-            const typename O::Stored* const at = keys + warp * per_warp;
-            for (int i = lane * W; i < (int)per_warp; i += 32 * W) {
-                const Pack<typename O::Stored, W> q = *(const Pack<typename O::Stored, W>*)(at + i);
-                if (!any_from(q, from)) continue;
+        const T* const x = (const T*)a.logits + row * v + s0;
+        auto key_at = [&](int64_t i) -> Key { return RESIDENT ? (Key)keys[i] : O::key(x[i]); };
+        const int64_t w0 = min(warp * per_warp, size), w1 = min(w0 + per_warp, size);
+        // f(key) for this warp's keys of at least `from`, which is 1 or more; in shared memory 16 bytes at a
+        // time, most of which have none once a border is known to be above
+        auto each = [&](Key from, auto&& f) {
+            if (RESIDENT) {
+                constexpr int W = 16 / sizeof(typename O::Stored);
+                const typename O::Stored* const at = keys + warp * per_warp;
+                for (int i = lane * W; i < (int)per_warp; i += 32 * W) {
+                    const Pack<typename O::Stored, W> q = *(const Pack<typename O::Stored, W>*)(at + i);
+                    if (!any_from(q, from)) continue;
 #pragma unroll
-                for (int j = 0; j < W; ++j)
-                    if (q.v[j] >= from) f((Key)q.v[j]);
+                    for (int j = 0; j < W; ++j)
+                        if (q.v[j] >= from) f((Key)q.v[j]);
+                }
+            } else {
+                for (int64_t i = w0 + lane; i < w1; i += 32) {
+                    const Key k = key_at(i);
+                    if (k >= from) f(k);
+                }
+            }
+        };
+
+        // the largest key
+        Key top = 0;
+        if (RESIDENT) {
+            // what is left of the slice behind the row: 0, below every key
+            constexpr int kTogether = 4;       // loads on their way at once
+            for (int i0 = tid * V; i0 < (int)slice; i0 += kTogether * kThreads * V) {
+                Pack<T, V> p[kTogether];
+#pragma unroll
+                for (int m = 0; m < kTogether; ++m)
+                    if (i0 + m * kThreads * V < size) p[m] = *(const Pack<T, V>*)(x + i0 + m * kThreads * V);
+#pragma unroll
+                for (int m = 0; m < kTogether; ++m) {
+                    const int i = i0 + m * kThreads * V;
+                    if (i >= (int)slice) break;
+                    Pack<typename O::Stored, V> q;
+#pragma unroll
+                    for (int j = 0; j < V; ++j) q.v[j] = 0;
+                    if (i < size) q = keys_of<T, V>(p[m]);
+                    *(Pack<typename O::Stored, V>*)(keys + i) = q;
+#pragma unroll
+                    for (int j = 0; j < V; ++j) top = q.v[j] > top ? q.v[j] : top;
+                }
             }
         } else {
-            for (int64_t i = w0 + lane; i < w1; i += 32) {
-                const Key k = key_at(i);
-                if (k >= from) f(k);
-            }
+            each(1, [&](Key k) { top = k > top ? k : top; });
         }
-    };
-
-    // the largest key
-    Key top = 0;
-    if (RESIDENT) {
-        // what is left of the slice behind the row: 0, below every key
-        constexpr int kTogether = 4;       // loads on their way at once
-        for (int i0 = tid * V; i0 < (int)slice; i0 += kTogether * kThreads * V) {
-            Pack<T, V> p[kTogether];
-#pragma unroll
-            for (int m = 0; m < kTogether; ++m)
-                if (i0 + m * kThreads * V < size) p[m] = *(const Pack<T, V>*)(x + i0 + m * kThreads * V);
-#pragma unroll
-            for (int m = 0; m < kTogether; ++m) {
-                const int i = i0 + m * kThreads * V;
-                if (i >= (int)slice) break;
-                Pack<typename O::Stored, V> q;
-#pragma unroll
-                for (int j = 0; j < V; ++j) q.v[j] = 0;
-                if (i < size) q = keys_of<T, V>(p[m]);
-                *(Pack<typename O::Stored, V>*)(keys + i) = q;
-#pragma unroll
-                for (int j = 0; j < V; ++j) top = q.v[j] > top ? q.v[j] : top;
-            }
+        for (int i = tid; i < 2 * kBins * M::kWords; i += kThreads) (&sh.bins[0][0])[i] = 0;
+        const Key own_top = top;
+        top = warp_max(top);
+        if (lane == 0) sh.top[warp] = top;
+        __syncthreads();
+        if (tid == 0) {
+            for (int w = 0; w < kWarps; ++w) top = sh.top[w] > top ? sh.top[w] : top;
+            sh.most = top;
         }
-    } else {
-        each(1, [&](Key k) { top = k > top ? k : top; });
-    }
-    for (int i = tid; i < 2 * kBins * M::kWords; i += kThreads) (&sh.bins[0][0])[i] = 0;
-    const Key own_top = top;
-    top = warp_max(top);
-    if (lane == 0) sh.top[warp] = top;
-    __syncthreads();
-    if (tid == 0) {
-        for (int w = 0; w < kWarps; ++w) top = sh.top[w] > top ? sh.top[w] : top;
-        sh.most = top;
-    }
-    cluster.sync();
-    top = 0;
-    if (lane < blocks) top = *cluster.map_shared_rank(&sh.most, lane);
-    top = warp_max(top);
-    const A most = O::value(top);
-    const A temp = (A)row_param(a.temperature, row);
-    const bool none = most == -INFINITY, greedy = !(temp > 0);
-    // differences are taken of halves, which do not overflow
-    const A half = most * A(0.5), scale = greedy ? A(0) : A(2 * 1.4426950408889634) / temp;
-    // only the largest has weight: it is infinite, or the temperature so small that its inverse is
-    const bool alone = greedy || most == INFINITY || scale == INFINITY;
-    // log2 of a weight, negated; infinite where the weight is 0
-    auto depth = [&](Key k) -> A {
-        const A e = O::value(k), d = (half - e * A(0.5)) * scale;
-        return k == top ? A(0) : alone || e == -INFINITY ? (A)INFINITY : d;
-    };
-    auto weight = [&](Key k) { return power(-depth(k)); };
-    auto mass = [&](Key k) { return M::of(weight(k), shift); };
-
-    // ---- borders ----
-    // The key at which the sum over the kept values in descending order reaches a target, the sum above
-    // it and its own: the number of values, or their weight.  `aim` gives the target for the sum of all.
-    int turn = 0;
-    Key edge = greedy ? top : 1;       // keys above the edge are kept, and the first `ties` at it
-    u64 ties = greedy ? 1 : ~0ULL, tied = ~0ULL;
-    struct Border { Key key; u64 above, own; };
-    // first round: bins of equal steps in log2 e, the last one open
-    const A wide = A(2) / (scale * kBinsPerOctave);
-    auto bin_of = [&](A depth) { return (int)fmin(depth * A(kBinsPerOctave), A(kBins - 1)); };
-    auto octave_bin = [&](Key k) { return bin_of(depth(k)); };
-    // keys not below and not above any of a bin, however bin and value were rounded
-    auto slack_of = [&](int bin) { return (fabs(most) + (A)(bin + 1) * wide) * (sizeof(A) == 8 ? A(1e-14) : A(1e-6)); };
-    auto bin_high = [&](int bin) { return bin > 0 ? min(top, O::at_least(most - (A)bin * wide + slack_of(bin))) : top; };
-    auto bin_low = [&](int bin) { return bin < kBins - 1 ? max((Key)1, O::at_most(most - (A)(bin + 1) * wide - slack_of(bin))) : (Key)1; };
-    // Adds up all blocks' histograms of this turn; the bin in which the sum from the top reaches
-    // target(sum of all), or -1; sh.before and sh.own are the sums above it and of it.
-    auto search = [&](auto by_weight, u64 above, auto&& target_of) -> int {
-        constexpr bool kWeight = decltype(by_weight)::value;
         cluster.sync();
-        unsigned* const bins = sh.bins[turn & 1];
-        const u64 own = M::template sum<!kWeight>(tid, blocks, [&](int q) { return cluster.map_shared_rank(bins, (rank + q) & (blocks - 1)); });
-        if (tid == 0) sh.found = -1;
-        u64 total;
-        const u64 before = above + block_prefix(own, sh.scan, &total);
-        const u64 target = target_of(total);
-        if (before < target && target <= before + own) {
-            sh.found = tid;
-            sh.before = before;
-            sh.own = own;
-        }
-        // the other histogram is free: all blocks have passed the barrier behind its last use
-        ++turn;
-        for (int i = tid; i < kBins * M::kWords; i += kThreads) sh.bins[turn & 1][i] = 0;
-        __syncthreads();
-        return sh.found;
-    };
-    auto border_of = [&](auto by_weight, Key floor, auto&& aim) -> Border {
-        constexpr bool kWeight = decltype(by_weight)::value;
-        int octave = -1, down = 0;
-        Key high = top, low = max(floor, edge);
-        u64 above = 0, target = 0;
-        // a round leaves 1/256 of the span or less: 9 are the most for 64-bit keys
-        for (int round = 0; round < 12; ++round) {
+        top = 0;
+        if (lane < blocks) top = *cluster.map_shared_rank(&sh.most, lane);
+        top = warp_max(top);
+        const A most = O::value(top);
+        const A temp = (A)row_param(a.temperature, row);
+        const bool none = most == -INFINITY, greedy = !(temp > 0);
+        // differences are taken of halves, which do not overflow
+        const A half = most * A(0.5), scale = greedy ? A(0) : A(2 * 1.4426950408889634) / temp;
+        // only the largest has weight: it is infinite, or the temperature so small that its inverse is
+        const bool alone = greedy || most == INFINITY || scale == INFINITY;
+        // log2 of a weight, negated; infinite where the weight is 0
+        auto depth = [&](Key k) -> A {
+            const A e = O::value(k), d = (half - e * A(0.5)) * scale;
+            return k == top ? A(0) : alone || e == -INFINITY ? (A)INFINITY : d;
+        };
+        auto weight = [&](Key k) { return power(-depth(k)); };
+        auto mass = [&](Key k) { return M::of(weight(k), shift); };
+
+        // ---- borders ----
+        // The key at which the sum over the kept values in descending order reaches a target, the sum above
+        // it and its own: the number of values, or their weight.  `aim` gives the target for the sum of all.
+        int turn = 0;
+        Key edge = greedy ? top : 1;       // keys above the edge are kept, and the first `ties` at it
+        u64 ties = greedy ? 1 : ~0ULL, tied = ~0ULL;
+        struct Border { Key key; u64 above, own; };
+        // first round: bins of equal steps in log2 e, the last one open
+        const A wide = A(2) / (scale * kBinsPerOctave);
+        auto bin_of = [&](A depth) { return (int)fmin(depth * A(kBinsPerOctave), A(kBins - 1)); };
+        auto octave_bin = [&](Key k) { return bin_of(depth(k)); };
+        // keys not below and not above any of a bin, however bin and value were rounded
+        auto slack_of = [&](int bin) { return (fabs(most) + (A)(bin + 1) * wide) * (sizeof(A) == 8 ? A(1e-14) : A(1e-6)); };
+        auto bin_high = [&](int bin) { return bin > 0 ? min(top, O::at_least(most - (A)bin * wide + slack_of(bin))) : top; };
+        auto bin_low = [&](int bin) { return bin < kBins - 1 ? max((Key)1, O::at_most(most - (A)(bin + 1) * wide - slack_of(bin))) : (Key)1; };
+        // Adds up all blocks' histograms of this turn; the bin in which the sum from the top reaches
+        // target(sum of all), or -1; sh.before and sh.own are the sums above it and of it.
+        auto search = [&](auto by_weight, u64 above, auto&& target_of) -> int {
+            constexpr bool kWeight = decltype(by_weight)::value;
+            cluster.sync();
             unsigned* const bins = sh.bins[turn & 1];
-            each(low, [&](Key k) {
-                if (k > high) return;
-                const A d = depth(k);
-                int bin = bin_of(d);
-                if (octave >= 0) {
-                    if (bin != octave) return;
-                    bin = (int)((high - k) >> down);
-                }
-                if (kWeight) M::add(bins, bin, power(-d), shift);
-                else M::count(bins, bin);
-            });
-            const int found = search(by_weight, above, [&](u64 total) { return target = octave < 0 ? aim(total) : target; });
-            if (found < 0) break;
-            above = sh.before;
-            const u64 mine = sh.own;
-            // the next search writes these behind barriers that every thread passes after this
-            if (octave < 0) {
-                octave = found;
-                high = bin_high(found);
-                low = max(low, bin_low(found));
-            } else {
-                high -= (Key)found << down;
-                const Key span = ((Key)1 << down) - 1;
-                low = high - low > span ? high - span : low;
+            const u64 own = M::template sum<!kWeight>(tid, blocks, [&](int q) { return cluster.map_shared_rank(bins, (rank + q) & (blocks - 1)); });
+            if (tid == 0) sh.found = -1;
+            u64 total;
+            const u64 before = above + block_prefix(own, sh.scan, &total);
+            const u64 target = target_of(total);
+            if (before < target && target <= before + own) {
+                sh.found = tid;
+                sh.before = before;
+                sh.own = own;
             }
-            if (low == high) return {high, above, mine};
-            const int bits = 64 - __clzll((u64)(high - low));    // of the span; bins of it have 9
-            down = bits > 9 ? bits - 9 : 0;
-        }
-        return {edge, above, 0};    // not reached: a target is never above the sum of all
-    };
-    // Writes down the token that `aim_of(total)` and the sums of kept weights decide on.
-    const double u = a.u_dtype == DT_F64 ? ((const double*)a.u)[row] : (double)((const float*)a.u)[row];
-    auto aim_of = [&](u64 total) {
-        const u64 aim = u > 0 ? (u >= 1 ? total : (u64)(u * (double)total)) : 0;
-        return aim >= total ? total - 1 : aim;
-    };
-    auto write = [&](Key k, int at, u64 total) {
-        a.token[row] = at;
-        const double e = k == top ? 0.0 : ((double)O::value(k) - (double)most) / (double)temp;
-        ((A*)a.logp)[row] = (A)(e - log((double)total / (double)(1ULL << shift)));
-    };
-    const A least = (A)fmin(row_param(a.min_p, row), 1.0);   // the largest logit stays
-    // The first block draws from the `count` largest values of the row, one a thread: the first `k` in
-    // their order, then top-p, min-p and the draw as everywhere.
-    auto draw_from = [&](int count, int from, int place, int k) {
-        Key key = 0;
-        int at = 0;
-        if (tid < count) {
-            key = cluster.map_shared_rank(sh.list_key, from)[place];
-            at = cluster.map_shared_rank(sh.list_at, from)[place];
-            sh.row_key[tid] = key;
-            sh.row_at[tid] = at;
-        }
-        __syncthreads();
-        int order = 0;
-        for (int i = 0; i < count; ++i) order += sh.row_key[i] > key || (sh.row_key[i] == key && sh.row_at[i] < at);
-        __syncthreads();
-        if (tid < count) {
-            sh.row_key[order] = key;
-            sh.row_at[order] = at;
-        }
-        __syncthreads();
-        const int kept_k = min(k, count);
-        key = tid < kept_k ? sh.row_key[tid] : 0;
-        at = sh.row_at[tid < kept_k ? tid : 0];
-        u64 m = tid < kept_k ? mass(key) : 0, sum, total;
-        const u64 before = block_prefix(m, sh.scan, &sum);
-        const double pp = row_param(a.top_p, row);
-        if (pp < 1) {
-            const double want = ceil(pp * (double)sum);
-            const u64 need = want >= 1 ? min((u64)want, sum) : 1;
-            if (before >= need) m = 0;
-        }
-        if (tid < kept_k && !(weight(key) >= least)) m = 0;
-        sh.row_mass[tid] = m;
-        block_prefix(m, sh.scan, &total);
-        __syncthreads();
-        u64 upto = 0;
-        for (int i = 0; i < kept_k; ++i) upto += sh.row_at[i] <= at ? sh.row_mass[i] : 0;
-        const u64 aim = aim_of(total);
-        if (m && upto - m <= aim && aim < upto) write(key, at, total);
-    };
-    bool short_list = false;
-    if (!greedy && !none) {
-        const double kk = row_param(a.top_k, row);
-        if (kk >= 1 && kk < (double)v) {
-            // the k-th largest of all threads' own largest keys is not above the k-th largest key: with it
-            // the first histogram is of a few values instead of all
-            Key floor = 1;
-            if (kk <= (double)(blocks * kThreads)) {
-                if (own_top) M::count(sh.bins[turn & 1], octave_bin(own_top));
-                if (tid == 0) sh.listed = 0;
-                const int found = search(std::false_type(), 0, [&](u64) { return (u64)kk; });
-                if (found >= 0) floor = bin_low(found);
-                if (RESIDENT && kk <= kList / 2 && found >= 0) {
-                    constexpr int W = 16 / sizeof(typename O::Stored);
-                    for (int i = tid * W; i < (int)slice; i += kThreads * W) {
-                        const Pack<typename O::Stored, W> q = *(const Pack<typename O::Stored, W>*)(keys + i);
-                        if (!any_from(q, floor)) continue;
+            // the other histogram is free: all blocks have passed the barrier behind its last use
+            ++turn;
+            for (int i = tid; i < kBins * M::kWords; i += kThreads) sh.bins[turn & 1][i] = 0;
+            __syncthreads();
+            return sh.found;
+        };
+        auto border_of = [&](auto by_weight, Key floor, auto&& aim) -> Border {
+            constexpr bool kWeight = decltype(by_weight)::value;
+            int octave = -1, down = 0;
+            Key high = top, low = max(floor, edge);
+            u64 above = 0, target = 0;
+            // a round leaves 1/256 of the span or less: 9 are the most for 64-bit keys
+            for (int round = 0; round < 12; ++round) {
+                unsigned* const bins = sh.bins[turn & 1];
+                each(low, [&](Key k) {
+                    if (k > high) return;
+                    const A d = depth(k);
+                    int bin = bin_of(d);
+                    if (octave >= 0) {
+                        if (bin != octave) return;
+                        bin = (int)((high - k) >> down);
+                    }
+                    if (kWeight) M::add(bins, bin, power(-d), shift);
+                    else M::count(bins, bin);
+                });
+                const int found = search(by_weight, above, [&](u64 total) { return target = octave < 0 ? aim(total) : target; });
+                if (found < 0) break;
+                above = sh.before;
+                const u64 mine = sh.own;
+                // the next search writes these behind barriers that every thread passes after this
+                if (octave < 0) {
+                    octave = found;
+                    high = bin_high(found);
+                    low = max(low, bin_low(found));
+                } else {
+                    high -= (Key)found << down;
+                    const Key span = ((Key)1 << down) - 1;
+                    low = high - low > span ? high - span : low;
+                }
+                if (low == high) return {high, above, mine};
+                const int bits = 64 - __clzll((u64)(high - low));    // of the span; bins of it have 9
+                down = bits > 9 ? bits - 9 : 0;
+            }
+            return {edge, above, 0};    // not reached: a target is never above the sum of all
+        };
+        // Writes down the token that `aim_of(total)` and the sums of kept weights decide on.
+        const double u = a.u_dtype == DT_F64 ? ((const double*)a.u)[row] : (double)((const float*)a.u)[row];
+        auto aim_of = [&](u64 total) {
+            const u64 aim = u > 0 ? (u >= 1 ? total : (u64)(u * (double)total)) : 0;
+            return aim >= total ? total - 1 : aim;
+        };
+        auto write = [&](Key k, int at, u64 total) {
+            a.token[row] = at;
+            const double e = k == top ? 0.0 : ((double)O::value(k) - (double)most) / (double)temp;
+            ((A*)a.logp)[row] = (A)(e - log((double)total / (double)(1ULL << shift)));
+        };
+        const A least = (A)fmin(row_param(a.min_p, row), 1.0);   // the largest logit stays
+        // The first block draws from the `count` largest values of the row, one a thread: the first `k` in
+        // their order, then top-p, min-p and the draw as everywhere.
+        auto draw_from = [&](int count, int from, int place, int k) {
+            Key key = 0;
+            int at = 0;
+            if (tid < count) {
+                key = cluster.map_shared_rank(sh.list_key, from)[place];
+                at = cluster.map_shared_rank(sh.list_at, from)[place];
+                sh.row_key[tid] = key;
+                sh.row_at[tid] = at;
+            }
+            __syncthreads();
+            int order = 0;
+            for (int i = 0; i < count; ++i) order += sh.row_key[i] > key || (sh.row_key[i] == key && sh.row_at[i] < at);
+            __syncthreads();
+            if (tid < count) {
+                sh.row_key[order] = key;
+                sh.row_at[order] = at;
+            }
+            __syncthreads();
+            const int kept_k = min(k, count);
+            key = tid < kept_k ? sh.row_key[tid] : 0;
+            at = sh.row_at[tid < kept_k ? tid : 0];
+            u64 m = tid < kept_k ? mass(key) : 0, sum, total;
+            const u64 before = block_prefix(m, sh.scan, &sum);
+            const double pp = row_param(a.top_p, row);
+            if (pp < 1) {
+                const double want = ceil(pp * (double)sum);
+                const u64 need = want >= 1 ? min((u64)want, sum) : 1;
+                if (before >= need) m = 0;
+            }
+            if (tid < kept_k && !(weight(key) >= least)) m = 0;
+            sh.row_mass[tid] = m;
+            block_prefix(m, sh.scan, &total);
+            __syncthreads();
+            u64 upto = 0;
+            for (int i = 0; i < kept_k; ++i) upto += sh.row_at[i] <= at ? sh.row_mass[i] : 0;
+            const u64 aim = aim_of(total);
+            if (m && upto - m <= aim && aim < upto) write(key, at, total);
+        };
+        bool short_list = false;
+        if (!greedy && !none) {
+            const double kk = row_param(a.top_k, row);
+            if (kk >= 1 && kk < (double)v) {
+                // the k-th largest of all threads' own largest keys is not above the k-th largest key: with it
+                // the first histogram is of a few values instead of all
+                Key floor = 1;
+                if (kk <= (double)(blocks * kThreads)) {
+                    if (own_top) M::count(sh.bins[turn & 1], octave_bin(own_top));
+                    if (tid == 0) sh.listed = 0;
+                    const int found = search(std::false_type(), 0, [&](u64) { return (u64)kk; });
+                    if (found >= 0) floor = bin_low(found);
+                    if (RESIDENT && kk <= kList / 2 && found >= 0) {
+                        constexpr int W = 16 / sizeof(typename O::Stored);
+                        for (int i = tid * W; i < (int)slice; i += kThreads * W) {
+                            const Pack<typename O::Stored, W> q = *(const Pack<typename O::Stored, W>*)(keys + i);
+                            if (!any_from(q, floor)) continue;
 #pragma unroll
-                        for (int j = 0; j < W; ++j) {
-                            if (q.v[j] < floor) continue;
-                            const int place = atomicAdd(&sh.listed, 1);
-                            if (place < kList) {
-                                sh.list_key[place] = q.v[j];
-                                sh.list_at[place] = (int)s0 + i + j;
+                            for (int j = 0; j < W; ++j) {
+                                if (q.v[j] < floor) continue;
+                                const int place = atomicAdd(&sh.listed, 1);
+                                if (place < kList) {
+                                    sh.list_key[place] = q.v[j];
+                                    sh.list_at[place] = (int)s0 + i + j;
+                                }
                             }
                         }
-                    }
-                    cluster.sync();
-                    int count = 0, from = 0, place = tid;
-                    for (int q = 0; q < blocks; ++q) {
-                        const int theirs = *cluster.map_shared_rank(&sh.listed, q);
-                        if (count <= tid && tid < count + theirs) {
-                            from = q;
-                            place = tid - count;
+                        cluster.sync();
+                        int count = 0, from = 0, place = tid;
+                        for (int q = 0; q < blocks; ++q) {
+                            const int theirs = *cluster.map_shared_rank(&sh.listed, q);
+                            if (count <= tid && tid < count + theirs) {
+                                from = q;
+                                place = tid - count;
+                            }
+                            count += theirs;
                         }
-                        count += theirs;
-                    }
-                    if (count <= kList) {     // the same in all blocks
-                        if (rank == 0) draw_from(count, from, place, (int)kk);
-                        short_list = true;
+                        if (count <= kList) {     // the same in all blocks
+                            if (rank == 0) draw_from(count, from, place, (int)kk);
+                            short_list = true;
+                        }
                     }
                 }
+                if (!short_list) {
+                    const Border b = border_of(std::false_type(), floor, [&](u64) { return (u64)kk; });
+                    edge = b.key;
+                    ties = (u64)kk - b.above;
+                    tied = b.own;
+                }
             }
-            if (!short_list) {
-            const Border b = border_of(std::false_type(), floor, [&](u64) { return (u64)kk; });
-            edge = b.key;
-            ties = (u64)kk - b.above;
-            tied = b.own;
+            const double pp = row_param(a.top_p, row);
+            if (pp < 1 && !short_list) {
+                u64 need = 0;
+                const Border b = border_of(std::true_type(), (Key)1, [&](u64 sum) {
+                    if (ties < tied) sum -= (tied - ties) * mass(edge);
+                    const double want = ceil(pp * (double)sum);
+                    need = want >= 1 ? min((u64)want, sum) : 1;
+                    return need;
+                });
+                const u64 m = mass(b.key), some = m ? (need - b.above + m - 1) / m : 1;
+                ties = b.key == edge && ties < some ? ties : some;
+                edge = b.key;
             }
         }
-        const double pp = row_param(a.top_p, row);
-        if (pp < 1 && !short_list) {
-            u64 need = 0;
-            const Border b = border_of(std::true_type(), (Key)1, [&](u64 sum) {
-                if (ties < tied) sum -= (tied - ties) * mass(edge);
-                const double want = ceil(pp * (double)sum);
-                need = want >= 1 ? min((u64)want, sum) : 1;
-                return need;
-            });
-            const u64 m = mass(b.key), some = m ? (need - b.above + m - 1) / m : 1;
-            ties = b.key == edge && ties < some ? ties : some;
-            edge = b.key;
-        }
-    }
 
-    // ---- the draw ----
-    if (!short_list) {
-    if (!(weight(edge) >= least)) ties = 0;
-    u64 mine = 0, at_edge = 0;
-    each(edge, [&](Key k) {
-        if (k == edge) {
-            ++at_edge;
-        } else {
-            const A e = weight(k);
-            if (e >= least) mine += M::of(e, shift);
-        }
-    });
-    mine = warp_sum(mine);
-    at_edge = warp_sum(at_edge);
-    if (lane == 0) {
-        sh.weight[warp] = mine;
-        sh.tied[warp] = at_edge;
-    }
-    cluster.sync();
-    // every block adds up all warps' weights in the order of the values
-    u64 theirs = 0, count = 0;
-    if (tid < blocks * kWarps) {
-        theirs = cluster.map_shared_rank(sh.weight, tid / kWarps)[tid % kWarps];
-        count = cluster.map_shared_rank(sh.tied, tid / kWarps)[tid % kWarps];
-    }
-    u64 total, unused;
-    const u64 tied_before = block_prefix(count, sh.scan, &unused);
-    if (ties > tied_before) theirs += min(count, ties - tied_before) * mass(edge);
-    const u64 before = block_prefix(theirs, sh.scan, &total);
-    const u64 aim = aim_of(total);
-    if (tid == 0) sh.found = -1;
-    __syncthreads();
-    if (!none && before <= aim && aim < before + theirs && tid / kWarps == rank) {
-        sh.found = tid % kWarps;
-        sh.before = before;
-        sh.extra = tied_before;
-    }
-    __syncthreads();
-    if (none && rank == 0 && tid == 0) {
-        a.token[row] = -1;
-        ((A*)a.logp)[row] = -INFINITY;
-    }
-    const int owner = sh.found;
-    if (owner >= 0) {
-        // the draw lies in the values of one warp of this block: all threads look for it, each in a
-        // piece of neighbouring values
-        const u64 first = sh.before, first_tie = sh.extra;
-        const int64_t o0 = min(owner * per_warp, size), o1 = min(o0 + per_warp, size), piece = (per_warp + kThreads - 1) / kThreads;
-        const int64_t i0 = min(o0 + tid * piece, o1), i1 = min(i0 + piece, o1);
-        u64 equal = 0, sum = 0;
-        for (int64_t i = i0; i < i1; ++i) equal += key_at(i) == edge;
-        const u64 tie0 = first_tie + block_prefix(equal, sh.scan, &unused);
-        auto walk = [&](auto&& stop) {
-            u64 tie = tie0, s = 0;
-            for (int64_t i = i0; i < i1; ++i) {
-                const Key k = key_at(i);
-                if (k == edge ? tie++ >= ties : k < edge || !(weight(k) >= least)) continue;
-                s += mass(k);
-                if (stop(s, i, k)) break;
-            }
-            return s;
-        };
-        sum = walk([](u64, int64_t, Key) { return false; });
-        const u64 here = first + block_prefix(sum, sh.scan, &unused);
-        if (here <= aim && aim < here + sum)
-            walk([&](u64 s, int64_t i, Key k) {
-                if (here + s <= aim) return false;
-                write(k, (int)(s0 + i), total);
-                return true;
+        // ---- the draw ----
+        if (!short_list) {
+            if (!(weight(edge) >= least)) ties = 0;
+            u64 mine = 0, at_edge = 0;
+            each(edge, [&](Key k) {
+                if (k == edge) {
+                    ++at_edge;
+                } else {
+                    const A e = weight(k);
+                    if (e >= least) mine += M::of(e, shift);
+                }
             });
-    }
-    }
-    cluster.sync();    // no block's shared memory goes, or has the next row, while another may read it
+            mine = warp_sum(mine);
+            at_edge = warp_sum(at_edge);
+            if (lane == 0) {
+                sh.weight[warp] = mine;
+                sh.tied[warp] = at_edge;
+            }
+            cluster.sync();
+            // every block adds up all warps' weights in the order of the values
+            u64 theirs = 0, count = 0;
+            if (tid < blocks * kWarps) {
+                theirs = cluster.map_shared_rank(sh.weight, tid / kWarps)[tid % kWarps];
+                count = cluster.map_shared_rank(sh.tied, tid / kWarps)[tid % kWarps];
+            }
+            u64 total, unused;
+            const u64 tied_before = block_prefix(count, sh.scan, &unused);
+            if (ties > tied_before) theirs += min(count, ties - tied_before) * mass(edge);
+            const u64 before = block_prefix(theirs, sh.scan, &total);
+            const u64 aim = aim_of(total);
+            if (tid == 0) sh.found = -1;
+            __syncthreads();
+            if (!none && before <= aim && aim < before + theirs && tid / kWarps == rank) {
+                sh.found = tid % kWarps;
+                sh.before = before;
+                sh.extra = tied_before;
+            }
+            __syncthreads();
+            if (none && rank == 0 && tid == 0) {
+                a.token[row] = -1;
+                ((A*)a.logp)[row] = -INFINITY;
+            }
+            const int owner = sh.found;
+            if (owner >= 0) {
+                // the draw lies in the values of one warp of this block: all threads look for it, each in a
+                // piece of neighbouring values
+                const u64 first = sh.before, first_tie = sh.extra;
+                const int64_t o0 = min(owner * per_warp, size), o1 = min(o0 + per_warp, size), piece = (per_warp + kThreads - 1) / kThreads;
+                const int64_t i0 = min(o0 + tid * piece, o1), i1 = min(i0 + piece, o1);
+                u64 equal = 0, sum = 0;
+                for (int64_t i = i0; i < i1; ++i) equal += key_at(i) == edge;
+                const u64 tie0 = first_tie + block_prefix(equal, sh.scan, &unused);
+                auto walk = [&](auto&& stop) {
+                    u64 tie = tie0, s = 0;
+                    for (int64_t i = i0; i < i1; ++i) {
+                        const Key k = key_at(i);
+                        if (k == edge ? tie++ >= ties : k < edge || !(weight(k) >= least)) continue;
+                        s += mass(k);
+                        if (stop(s, i, k)) break;
+                    }
+                    return s;
+                };
+                sum = walk([](u64, int64_t, Key) { return false; });
+                const u64 here = first + block_prefix(sum, sh.scan, &unused);
+                if (here <= aim && aim < here + sum)
+                    walk([&](u64 s, int64_t i, Key k) {
+                        if (here + s <= aim) return false;
+                        write(k, (int)(s0 + i), total);
+                        return true;
+                    });
+            }
+        }
+        cluster.sync();    // no block's shared memory goes, or has the next row, while another may read it
     }
 }
 
