@@ -8,7 +8,7 @@
 // A temperature that is not above 0 keeps the first of the largest logits alone.
 // The token is the first in index order whose running sum of kept e exceeds u times their total.
 //
-// The sums are held as 64-bit integers, rint(e 2^s) with s such that no row overflows: they do not
+// The sums are held as 64-bit integers, e 2^s rounded to one, with s such that no row overflows: they do not
 // depend on the order of the additions, so every way of splitting a row gives the same token, and
 // the first two filters come down to one border in the order of the logits, (key, number of ties kept).
 // NaN counts as -infinity.  A row with +infinities draws among them alone.
@@ -18,7 +18,7 @@
 // A cluster of up to 8 blocks has a row, each block a slice of it in shared memory as
 // integer keys in the order of the values, read from HBM once.  A border is found by histograms: the
 // first over steps of 1/16 in log2 e, the next over what the bin with the border spans in key space,
-// 512 times finer each time, until a bin is one key.  Every block adds up all blocks' histograms
+// 512 times finer each time, until a bin is one key or few values are left, which are ordered.  Every block adds up all blocks' histograms
 // (distributed shared memory), so that one cluster barrier a round is enough.  A top-k of a few hundred
 // leaves few values above a bound that is found from each thread's largest key; those are brought
 // together and ordered by counting, and the rest of the work is on that list.
@@ -46,7 +46,7 @@ namespace {
 typedef unsigned long long u64;
 
 constexpr int kThreads = 512, kWarps = kThreads / 32, kBins = kThreads, kMostBlocks = 8;
-constexpr int kBinsPerOctave = 16, kGrain = 256, kList = kThreads;
+constexpr int kBinsPerOctave = 16, kGrain = 8, kList = kThreads;
 
 // Integers in the order of the values; -0 and 0 are one value, NaN the lowest.
 template <typename T> struct Order;
@@ -134,9 +134,9 @@ __device__ __forceinline__ float power(float v) {
 }
 __device__ __forceinline__ double power(double v) { return exp2(v); }
 
-// Weights e of 0 to 1 as integers.  WIDE: 64 bits at once, rint(e 2^shift).  Else three limbs of 15 bits,
-// whose sums over a slice of up to 2^15 values fit the 32 bits that shared memory can add to at once,
-// and whose sum over 8 slices fits 64.
+// Weights e of 0 to 1 as integers.  WIDE: 64 bits at once, rint(e 2^shift).  Else floor(e 2^45) in three limbs
+// of 12, 17 and 17 bits, whose sums over a slice of up to 2^15 values fit the 32 bits that shared memory can add
+// to at once, and whose sum over 8 slices fits 64.
 // A histogram is an array of bins of 64 bits, or three arrays of the limbs' sums.
 template <bool WIDE> struct Mass;
 template <> struct Mass<true> {
@@ -150,21 +150,31 @@ template <> struct Mass<true> {
         for (int q = 0; q < blocks; ++q) own += ((const u64*)bins_of(q))[i];
         return own;
     }
+    // a thread's sum
+    struct Sum {
+        u64 s = 0;
+        template <typename A> __device__ __forceinline__ void add(A e, int shift) { s += of(e, shift); }
+        __device__ __forceinline__ u64 total() const { return s; }
+    };
 };
 template <> struct Mass<false> {
     static constexpr int kWords = 3;
-    // e 2^45 to the nearest: the significand shifted by the exponent, without a conversion's slow unit
-    __device__ static u64 of(float e, int) {
-        const unsigned bits = __float_as_uint(e), significand = (bits & 0x7fffffu) | 0x800000u;
-        const int up = (int)(bits >> 23) - 105;       // 1 is 2^23 2^22
-        if (up >= 0) return (u64)significand << up;
-        return up > -26 ? (significand + (1u << (-up - 1))) >> -up : 0;
+    struct Limbs { unsigned high, mid, low; };
+    // Added to 2^12 (2^-5, 2^-22) and rounded down, a value below 1 (2^-11, 2^-28) leaves its multiple of 2^-11
+    // (2^-28, 2^-45) in the last bits; what is taken off it is exact.  No branches, no conversions.
+    __device__ __forceinline__ static Limbs limbs(float e) {
+        const float h = __fadd_rd(e, 0x1p12f), r = __fadd_rn(e, __fadd_rn(0x1p12f, -h));
+        const float m = __fadd_rd(r, 0x1p-5f), q = __fadd_rn(r, __fadd_rn(0x1p-5f, -m));
+        const float l = __fadd_rd(q, 0x1p-22f);
+        return {__float_as_uint(h) & 0xfffu, __float_as_uint(m) & 0x1ffffu, __float_as_uint(l) & 0x1ffffu};
     }
-    __device__ static void add(unsigned* bins, int bin, float e, int) {
-        const u64 m = of(e, 0);
-        if (m >> 30) atomicAdd(bins + bin, (unsigned)(m >> 30));     // the largest few
-        atomicAdd(bins + kBins + bin, (unsigned)(m >> 15) & 0x7fffu);
-        atomicAdd(bins + 2 * kBins + bin, (unsigned)m & 0x7fffu);
+    __device__ __forceinline__ static u64 whole(Limbs p) { return ((u64)p.high << 34) + ((u64)p.mid << 17) + p.low; }
+    __device__ static u64 of(float e, int) { return whole(limbs(e)); }
+    __device__ __forceinline__ static void add(unsigned* bins, int bin, float e, int) {
+        const Limbs p = limbs(e);
+        if (p.high) atomicAdd(bins + bin, p.high);     // weights of 2^-11 and more
+        atomicAdd(bins + kBins + bin, p.mid);
+        atomicAdd(bins + 2 * kBins + bin, p.low);
     }
     __device__ static void count(unsigned* bins, int bin) { atomicAdd(bins + 2 * kBins + bin, 1u); }
     template <bool COUNT, typename F> __device__ static u64 sum(int i, int blocks, F&& bins_of) {
@@ -180,10 +190,21 @@ template <> struct Mass<false> {
             u64 limb = 0;
 #pragma unroll
             for (int q = 0; q < kMostBlocks; ++q) limb += w[k][q];
-            own += COUNT ? limb : limb << 15 * (2 - k);
+            own += COUNT ? limb : limb << 17 * (2 - k);
         }
         return own;
     }
+    // a thread's sum, of up to 2^15 values
+    struct Sum {
+        Limbs s = {0, 0, 0};
+        __device__ __forceinline__ void add(float e, int) {
+            const Limbs p = limbs(e);
+            s.high += p.high;
+            s.mid += p.mid;
+            s.low += p.low;
+        }
+        __device__ __forceinline__ u64 total() const { return whole(s); }
+    };
 };
 
 template <typename T, bool WIDE>
@@ -194,10 +215,11 @@ struct SampleShared {
     u64 tied[kWarps];                                          // ... and values at the border
     typename Order<T>::Key top[kWarps], most;
     u64 before, own, extra;                                    // what a search has found
+    typename Order<T>::Key border;
     int found;
-    // a short list of the largest values, of this block and then (in the first block) of the row
-    int listed;
-    typename Order<T>::Key list_key[kList], row_key[kList];
+    // a short list of values, of this block and then of the row; two rounds' counters
+    int listed[2];
+    alignas(16) typename Order<T>::Key list_key[kList], row_key[kList];
     int list_at[kList], row_at[kList];
     u64 row_mass[kList];
 };
@@ -226,7 +248,7 @@ __device__ __forceinline__ u64 block_prefix(u64 v, u64* sm, u64* total) {
 }
 
 // One cluster a row.  RESIDENT: a block's slice fits its shared memory; else it is read from L2 each time.
-// V: values of one load.  A warp has `per_warp` neighbouring values (a multiple of kGrain) of the slice.
+// V: values of one load.  A warp has `per_warp` neighbouring values (a multiple of kGrain: 16 bytes) of the slice.
 template <typename T, int V, bool WIDE, bool RESIDENT>
 __global__ void __launch_bounds__(kThreads, sizeof(T) == 8 ? 1 : 2) sample_kernel(SampleArgs a, int64_t per_warp, int shift) {
     using A = typename Acc<T>::type;
@@ -294,6 +316,7 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 8 ? 1 : 2) sample_kerne
             each(1, [&](Key k) { top = k > top ? k : top; });
         }
         for (int i = tid; i < 2 * kBins * M::kWords; i += kThreads) (&sh.bins[0][0])[i] = 0;
+        if (tid < 2) sh.listed[tid] = 0;
         const Key own_top = top;
         top = warp_max(top);
         if (lane == 0) sh.top[warp] = top;
@@ -336,11 +359,33 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 8 ? 1 : 2) sample_kerne
         auto slack_of = [&](int bin) { return (fabs(most) + (A)(bin + 1) * wide) * (sizeof(A) == 8 ? A(1e-14) : A(1e-6)); };
         auto bin_high = [&](int bin) { return bin > 0 ? min(top, O::at_least(most - (A)bin * wide + slack_of(bin))) : top; };
         auto bin_low = [&](int bin) { return bin < kBins - 1 ? max((Key)1, O::at_most(most - (A)(bin + 1) * wide - slack_of(bin))) : (Key)1; };
-        // Adds up all blocks' histograms of this turn; the bin in which the sum from the top reaches
+        // to the other histogram and counter, which are free: all blocks have passed the barrier behind their last use
+        auto advance = [&]() {
+            ++turn;
+            for (int i = tid; i < kBins * M::kWords; i += kThreads) sh.bins[turn & 1][i] = 0;
+            if (tid == 0) sh.listed[turn & 1] = 0;
+            __syncthreads();
+        };
+        // Values listed by all blocks in this turn, behind a barrier of the cluster; this thread's is the
+        // `place`th of block `from`.
+        auto listed = [&](int& from, int& place) {
+            const int each_of = lane < blocks ? *cluster.map_shared_rank(&sh.listed[turn & 1], lane) : 0;
+            int count = 0;
+#pragma unroll
+            for (int q = 0; q < kMostBlocks; ++q) {
+                const int theirs = __shfl_sync(0xffffffffu, each_of, q);
+                if (count <= tid && tid < count + theirs) {
+                    from = q;
+                    place = tid - count;
+                }
+                count += theirs;
+            }
+            return count;
+        };
+        // Adds up all blocks' histograms of this turn, behind a barrier of the cluster; the bin in which the sum from the top reaches
         // target(sum of all), or -1; sh.before and sh.own are the sums above it and of it.
         auto search = [&](auto by_weight, u64 above, auto&& target_of) -> int {
             constexpr bool kWeight = decltype(by_weight)::value;
-            cluster.sync();
             unsigned* const bins = sh.bins[turn & 1];
             const u64 own = M::template sum<!kWeight>(tid, blocks, [&](int q) { return cluster.map_shared_rank(bins, (rank + q) & (blocks - 1)); });
             if (tid == 0) sh.found = -1;
@@ -352,10 +397,7 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 8 ? 1 : 2) sample_kerne
                 sh.before = before;
                 sh.own = own;
             }
-            // the other histogram is free: all blocks have passed the barrier behind its last use
-            ++turn;
-            for (int i = tid; i < kBins * M::kWords; i += kThreads) sh.bins[turn & 1][i] = 0;
-            __syncthreads();
+            advance();
             return sh.found;
         };
         auto border_of = [&](auto by_weight, Key floor, auto&& aim) -> Border {
@@ -363,6 +405,63 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 8 ? 1 : 2) sample_kerne
             int octave = -1, down = 0;
             Key high = top, low = max(floor, edge);
             u64 above = 0, target = 0;
+            // The border among the listed values, one a thread (in every block): they are put in descending
+            // order by counting, and their sums taken in it.
+            auto in_list = [&](int count, int from, int place) -> Border {
+                constexpr int W = 16 / sizeof(Key);
+                const Key key = tid < count ? cluster.map_shared_rank(sh.list_key, from)[place] : 0;
+                sh.row_key[tid] = key;
+                if (tid == 0) sh.found = 0;
+                __syncthreads();
+                // greater ones are in front, and equal ones of lower threads; behind the list there are zeros
+                int order = 0;
+                if (tid < count) {
+                    const int w0 = tid - lane;
+#pragma unroll 4
+                    for (int i = 0; i < w0; i += W) {
+                        const Pack<Key, W> p = *(const Pack<Key, W>*)(sh.row_key + i);
+#pragma unroll
+                        for (int j = 0; j < W; ++j) order += p.v[j] >= key;
+                    }
+#pragma unroll
+                    for (int i = 0; i < 32; i += W) {
+                        const Pack<Key, W> p = *(const Pack<Key, W>*)(sh.row_key + w0 + i);
+#pragma unroll
+                        for (int j = 0; j < W; ++j) order += (p.v[j] > key) | ((p.v[j] == key) & (i + j < lane));
+                    }
+#pragma unroll 4
+                    for (int i = w0 + 32; i < count; i += W) {
+                        const Pack<Key, W> p = *(const Pack<Key, W>*)(sh.row_key + i);
+#pragma unroll
+                        for (int j = 0; j < W; ++j) order += p.v[j] > key;
+                    }
+                }
+                __syncthreads();
+                sh.row_mass[tid] = 0;
+                if (tid < count) sh.row_key[order] = key;
+                __syncthreads();
+                if (tid < count) sh.row_mass[order] = kWeight ? mass(key) : 1;
+                __syncthreads();
+                const u64 m = sh.row_mass[tid];
+                u64 all;
+                const u64 before = above + block_prefix(m, sh.scan, &all);
+                if (before < target && target <= before + m) {
+                    const Key k = sh.row_key[tid];
+                    auto places = [&](auto&& in_front) {      // values of which this holds, which are the first ones
+                        int n = 0;
+                        for (int step = kList / 2; step > 0; step /= 2)
+                            if (n + step <= count && in_front(sh.row_key[n + step - 1])) n += step;
+                        return n < count && in_front(sh.row_key[n]) ? n + 1 : n;
+                    };
+                    const int greater = places([&](Key q) { return q > k; }), least = places([&](Key q) { return q >= k; });
+                    sh.border = k;
+                    sh.before = before - (u64)(tid - greater) * m;
+                    sh.own = (u64)(least - greater) * m;
+                    sh.found = 1;
+                }
+                advance();
+                return sh.found ? Border{sh.border, sh.before, sh.own} : Border{edge, above, 0};
+            };
             // a round leaves 1/256 of the span or less: 9 are the most for 64-bit keys
             for (int round = 0; round < 12; ++round) {
                 unsigned* const bins = sh.bins[turn & 1];
@@ -372,11 +471,19 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 8 ? 1 : 2) sample_kerne
                     int bin = bin_of(d);
                     if (octave >= 0) {
                         if (bin != octave) return;
+                        const int place = atomicAdd(&sh.listed[turn & 1], 1);
+                        if (place < kList) sh.list_key[place] = k;
                         bin = (int)((high - k) >> down);
                     }
                     if (kWeight) M::add(bins, bin, power(-d), shift);
                     else M::count(bins, bin);
                 });
+                cluster.sync();
+                if (octave >= 0) {
+                    int from = 0, place = 0;
+                    const int count = listed(from, place);
+                    if (count <= kList) return in_list(count, from, place);      // the same in all blocks
+                }
                 const int found = search(by_weight, above, [&](u64 total) { return target = octave < 0 ? aim(total) : target; });
                 if (found < 0) break;
                 above = sh.before;
@@ -422,7 +529,11 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 8 ? 1 : 2) sample_kerne
             }
             __syncthreads();
             int order = 0;
-            for (int i = 0; i < count; ++i) order += sh.row_key[i] > key || (sh.row_key[i] == key && sh.row_at[i] < at);
+#pragma unroll 8
+            for (int i = 0; i < (tid < count ? count : 0); ++i) {
+                const Key k = sh.row_key[i];
+                order += (k > key) | ((k == key) & (sh.row_at[i] < at));
+            }
             __syncthreads();
             if (tid < count) {
                 sh.row_key[order] = key;
@@ -445,7 +556,11 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 8 ? 1 : 2) sample_kerne
             block_prefix(m, sh.scan, &total);
             __syncthreads();
             u64 upto = 0;
-            for (int i = 0; i < kept_k; ++i) upto += sh.row_at[i] <= at ? sh.row_mass[i] : 0;
+#pragma unroll 8
+            for (int i = 0; i < (m ? kept_k : 0); ++i) {
+                const u64 w = sh.row_mass[i];
+                upto += sh.row_at[i] <= at ? w : 0;
+            }
             const u64 aim = aim_of(total);
             if (m && upto - m <= aim && aim < upto) write(key, at, total);
         };
@@ -458,18 +573,17 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 8 ? 1 : 2) sample_kerne
                 Key floor = 1;
                 if (kk <= (double)(blocks * kThreads)) {
                     if (own_top) M::count(sh.bins[turn & 1], octave_bin(own_top));
-                    if (tid == 0) sh.listed = 0;
+                    cluster.sync();
                     const int found = search(std::false_type(), 0, [&](u64) { return (u64)kk; });
                     if (found >= 0) floor = bin_low(found);
                     if (RESIDENT && kk <= kList / 2 && found >= 0) {
-                        constexpr int W = 16 / sizeof(typename O::Stored);
-                        for (int i = tid * W; i < (int)slice; i += kThreads * W) {
-                            const Pack<typename O::Stored, W> q = *(const Pack<typename O::Stored, W>*)(keys + i);
-                            if (!any_from(q, floor)) continue;
+                        // most threads have loaded none
+                        for (int i = tid * V; own_top >= floor && i < (int)slice; i += kThreads * V) {
+                            const Pack<typename O::Stored, V> q = *(const Pack<typename O::Stored, V>*)(keys + i);
 #pragma unroll
-                            for (int j = 0; j < W; ++j) {
+                            for (int j = 0; j < V; ++j) {
                                 if (q.v[j] < floor) continue;
-                                const int place = atomicAdd(&sh.listed, 1);
+                                const int place = atomicAdd(&sh.listed[turn & 1], 1);
                                 if (place < kList) {
                                     sh.list_key[place] = q.v[j];
                                     sh.list_at[place] = (int)s0 + i + j;
@@ -477,15 +591,8 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 8 ? 1 : 2) sample_kerne
                             }
                         }
                         cluster.sync();
-                        int count = 0, from = 0, place = tid;
-                        for (int q = 0; q < blocks; ++q) {
-                            const int theirs = *cluster.map_shared_rank(&sh.listed, q);
-                            if (count <= tid && tid < count + theirs) {
-                                from = q;
-                                place = tid - count;
-                            }
-                            count += theirs;
-                        }
+                        int from = 0, place = 0;
+                        const int count = listed(from, place);
                         if (count <= kList) {     // the same in all blocks
                             if (rank == 0) draw_from(count, from, place, (int)kk);
                             short_list = true;
@@ -517,16 +624,17 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 8 ? 1 : 2) sample_kerne
         // ---- the draw ----
         if (!short_list) {
             if (!(weight(edge) >= least)) ties = 0;
-            u64 mine = 0, at_edge = 0;
+            typename M::Sum above;
+            u64 at_edge = 0;
             each(edge, [&](Key k) {
                 if (k == edge) {
                     ++at_edge;
                 } else {
                     const A e = weight(k);
-                    if (e >= least) mine += M::of(e, shift);
+                    if (e >= least) above.add(e, shift);
                 }
             });
-            mine = warp_sum(mine);
+            const u64 mine = warp_sum(above.total());
             at_edge = warp_sum(at_edge);
             if (lane == 0) {
                 sh.weight[warp] = mine;
