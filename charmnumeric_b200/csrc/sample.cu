@@ -25,9 +25,13 @@
 //
 // 128 rows of 131072 in 16 bits, top-k 50, top-p 0.9, min-p 0.02: a block a row without shared memory 1592 us;
 // clusters with keys in shared memory 226; histograms read in wide, coalesced pieces 136; rows looped over
-// by resident clusters (a cluster starts slower than a row that follows another in it) 96; the short list
-// 54 us.  One row of 32768 with top-p alone: 419, 102, 27, 27, 24 us.
-// 1024 threads, and passes without branches, were slower.
+// by resident clusters (a cluster starts slower than a row that follows another in it) 96; the short list 54;
+// looked for by the threads that have loaded its values 51 us (floor 5).
+// One row of 32768 in 32 bits with top-p 0.95: 419, 102, 27 us; the last rounds as an ordered list 20.5 us.
+// 37 rows of 50021 in 32 bits with top-p 0.98: 649 to 45 us, of it the first histogram and the draw, each a
+// weight for every value, 6 and 5, the barriers and prefix sums between them most of the rest.
+// Slower: 1024 threads; weights of four neighbouring values made together before they are used (47 us); the
+// draw's prefix sums in one warp alone (47 us).
 #include <cooperative_groups.h>
 
 #include <algorithm>
@@ -735,7 +739,7 @@ cudaError_t sample(const SampleArgs& a, int sm_count, cudaStream_t s) {
     while ((1LL << (62 - shift)) < a.v) --shift;
     if (a.rows * blocks >= (1LL << 31)) return cudaErrorInvalidValue;
     constexpr int V = 16 / sizeof(T);
-    if (kDouble) {
+    if constexpr (kDouble) {
         if (slice > kSlice) return launch<T, 1, true, false>(a, blocks, per_warp, shift, sm_count, s);
         return a.v % V == 0 ? launch<T, V, true, true>(a, blocks, per_warp, shift, sm_count, s) : launch<T, 1, true, true>(a, blocks, per_warp, shift, sm_count, s);
     } else {
