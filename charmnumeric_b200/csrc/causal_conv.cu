@@ -5,11 +5,12 @@
 // X continues x to negative times with the state, the k - 1 inputs before the first.  The new state
 // is the last k - 1 rows of X; behind the end of a sequence y is 0.
 //
-// Bound by HBM: x is read and y written once.  A thread has V neighbouring channels (16 bytes where the
-// channels allow) and walks a run of steps with the last inputs in registers, so that an input is
-// loaded once but for the k - 1 in front of a run.
-// 4 x 4096 x 4096 channels, width 4, in 16 bits, of random lengths (up to 268 MB, 41 us): 348 us with a channel
-// a thread, 69 with 16 bytes and inputs in registers, 53 to 60 with filters loaded in 16-byte pieces too.
+// Bound by HBM: x is read and y written once.  A thread has V neighbouring channels (four where the channels
+// allow, two of 64 bits) and walks a run of steps with the last inputs in registers, so that an input is
+// loaded once but for the k - 1 in front of a run; eight steps' inputs are requested together.
+// 4 x 4096 x 4096 channels, width 4, in 16 bits, full lengths (268 MB, floor 41 us): 59 us.  Eight channels and
+// four steps together, which hold more of the registers for fewer blocks an SM, 92; four and four 62; runs of
+// 64 steps as 32; 16 steps together and partial groups with a condition on every step 83 and more.
 // 96 single tokens of 4100 channels in 32 bits: 12.3 to 6.2 us, most of it the launch.
 #include <algorithm>
 
@@ -23,7 +24,7 @@ using namespace seq;
 
 namespace {
 
-constexpr int kThreads = 128, kTogether = 4;    // steps whose inputs are requested together
+constexpr int kThreads = 128;
 
 __device__ __forceinline__ float silu(float v) {
     float e, r;
@@ -33,17 +34,19 @@ __device__ __forceinline__ float silu(float v) {
 }
 __device__ __forceinline__ double silu(double v) { return v / (1.0 + exp(-v)); }
 
-// K is the width or more: filters are padded in front with zeros, over inputs that are zero there
-template <typename T, int V, int K>
-__global__ void __launch_bounds__(kThreads) causal_conv_kernel(CausalConvArgs a, int64_t run, int64_t runs) {
+// K is the width or more: filters are padded in front with zeros, over inputs that are zero there.  Five
+// blocks an SM where the filters and inputs leave the registers for it.  TOGETHER: steps whose inputs are
+// requested together, 8, or 1 for single tokens (with the others' registers and code 10.2 instead of 6.2 us).
+template <typename T, int V, int K, int TOGETHER>
+__global__ void __launch_bounds__(kThreads, TOGETHER == 1 ? 1 : K <= 4 && sizeof(T) <= 4 ? 5 : 3) causal_conv_kernel(CausalConvArgs a, int64_t run, int64_t runs) {
     using A = typename Acc<T>::type;
     const int64_t id = (int64_t)blockIdx.x * kThreads + threadIdx.x, across = a.d / V;
     if (id >= across * runs) return;
     const int64_t c = id % across * V, t0 = id / across * run, t1 = min(t0 + run, a.t);
     const int pad = K - a.k;
     A w[K][V], bias[V];
-    if constexpr (V * sizeof(T) == 16 && K < kMaxConvWidth) {
-        // the filters of V channels are K pieces of 16 bytes
+    if constexpr (V * sizeof(T) >= 8 && K < kMaxConvWidth) {
+        // the filters of V channels are K pieces of V values
         T f[K * V];
 #pragma unroll
         for (int i = 0; i < K; ++i) {
@@ -89,12 +92,18 @@ __global__ void __launch_bounds__(kThreads) causal_conv_kernel(CausalConvArgs a,
         int64_t t = t0;
         if (t < live) {
             A win[K - 1][V];
+            Pack<T, V> first[K - 1];
+            if (t0 >= K - 1) {
 #pragma unroll
-            for (int j = 0; j < K - 1; ++j) {
-                const Pack<T, V> p = input(t0 - K + 1 + j);
+                for (int j = 0; j < K - 1; ++j) first[j] = *(const Pack<T, V>*)(xs + (t0 - K + 1 + j) * a.d);
+            } else {
 #pragma unroll
-                for (int v = 0; v < V; ++v) win[j][v] = widen(p.v[v]);
+                for (int j = 0; j < K - 1; ++j) first[j] = input(t0 - K + 1 + j);
             }
+#pragma unroll
+            for (int j = 0; j < K - 1; ++j)
+#pragma unroll
+                for (int v = 0; v < V; ++v) win[j][v] = widen(first[j].v[v]);
             auto step = [&](const Pack<T, V>& p, T* to) {
                 Pack<T, V> y;
 #pragma unroll
@@ -113,14 +122,26 @@ __global__ void __launch_bounds__(kThreads) causal_conv_kernel(CausalConvArgs a,
             };
             const T* from = xs + t * a.d;
             T* to = ys + t * a.d;
-            for (; t + kTogether <= live; t += kTogether) {
-                Pack<T, V> p[kTogether];
+            if constexpr (TOGETHER == 1) {
+                for (; t < live; ++t, from += a.d, to += a.d) step(*(const Pack<T, V>*)from, to);
+            } else {
+                Pack<T, V> p[TOGETHER];
+                for (; t + TOGETHER <= live; t += TOGETHER) {
 #pragma unroll
-                for (int i = 0; i < kTogether; ++i, from += a.d) p[i] = *(const Pack<T, V>*)from;
+                    for (int i = 0; i < TOGETHER; ++i, from += a.d) p[i] = *(const Pack<T, V>*)from;
 #pragma unroll
-                for (int i = 0; i < kTogether; ++i, to += a.d) step(p[i], to);
+                    for (int i = 0; i < TOGETHER; ++i, to += a.d) step(p[i], to);
+                }
+                // the last few, together too
+                const int rest = (int)(live - t);
+#pragma unroll
+                for (int i = 0; i < TOGETHER - 1; ++i, from += a.d)
+                    if (i < rest) p[i] = *(const Pack<T, V>*)from;
+#pragma unroll
+                for (int i = 0; i < TOGETHER - 1; ++i, to += a.d)
+                    if (i < rest) step(p[i], to);
+                t = live;
             }
-            for (; t < live; ++t, from += a.d, to += a.d) step(*(const Pack<T, V>*)from, to);
         }
         for (; t < t1; ++t) *(Pack<T, V>*)(ys + t * a.d) = zero;
         if (t0 == 0) {
@@ -140,7 +161,9 @@ cudaError_t conv(const CausalConvArgs& a, int sm_count, cudaStream_t s) {
     while (run > 8 && across * a.b * ((a.t + run - 1) / run) < threads) run /= 2;
     const int64_t runs = std::max<int64_t>((a.t + run - 1) / run, 1), blocks = (across * runs + kThreads - 1) / kThreads;
     if (blocks >= (1LL << 31)) return cudaErrorInvalidValue;
-    causal_conv_kernel<T, V, K><<<dim3((unsigned)blocks, (unsigned)std::min<int64_t>(a.b, 65535)), kThreads, 0, s>>>(a, run, runs);
+    const dim3 grid((unsigned)blocks, (unsigned)std::min<int64_t>(a.b, 65535));
+    if (a.t == 1) causal_conv_kernel<T, V, K, 1><<<grid, kThreads, 0, s>>>(a, run, runs);
+    else causal_conv_kernel<T, V, K, 8><<<grid, kThreads, 0, s>>>(a, run, runs);
     return cudaGetLastError();
 }
 
@@ -156,7 +179,7 @@ cudaError_t conv(const CausalConvArgs& a, int sm_count, cudaStream_t s) {
 
 template <typename T>
 cudaError_t conv(const CausalConvArgs& a, int sm_count, cudaStream_t s) {
-    constexpr int V = 16 / sizeof(T);
+    constexpr int V = sizeof(T) == 8 ? 2 : 4;
     if (a.d % V == 0) return conv<T, V>(a, sm_count, s);
     if (V > 2 && a.d % 2 == 0) return conv<T, 2>(a, sm_count, s);
     return conv<T, 1>(a, sm_count, s);
