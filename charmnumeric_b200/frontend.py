@@ -372,6 +372,8 @@ class _ArrayOps:
         if _is_storage(self.dtype) or (isinstance(rhs, _ArrayOps) and _is_storage(rhs.dtype)):
             # no generated kernel takes these: a fill or a copy, its own node
             if not isinstance(rhs, _ArrayOps):
+                if self.dtype == np.dtype("int8") and not -128 <= rhs <= 127:
+                    raise OverflowError(f"{rhs} is no int8 value")
                 _record(_Op("fill", wire.OP_SET_REGION, self._info, [rhs], region=region))
                 return
             if rhs.dtype != self.dtype:

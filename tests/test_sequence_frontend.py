@@ -225,3 +225,14 @@ def test_the_profiled_kernels_built_ahead_of_time_are_the_ones_in_the_tree():
     now = hashlib.sha256((csrc / "kernels.cu").read_bytes() + (csrc / "kernels.hpp").read_bytes()).hexdigest()[:8]
     entries = json.loads((root / "profiles" / "dram_traffic.json").read_text())["kernels"]
     assert [e["code"] for e in entries if "matvec" in e["match"]] == ["#" + now]
+
+
+@pytest.mark.parametrize("value", [128, -129, 300.5, float("nan"), float("inf")])
+def test_int8_arrays_are_not_filled_with_what_they_cannot_hold(value):
+    with pytest.raises(OverflowError):
+        cnp.full((2,), value, dtype="int8")
+    a = z(2, dtype="int8")
+    with pytest.raises(OverflowError):
+        a[:1] = value
+    a[:1] = -128
+    a[1:] = 127
