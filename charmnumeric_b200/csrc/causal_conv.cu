@@ -8,9 +8,12 @@
 // Bound by HBM: x is read and y written once.  A thread has V neighbouring channels (four where the channels
 // allow, two of 64 bits) and walks a run of steps with the last inputs in registers, so that an input is
 // loaded once but for the k - 1 in front of a run; eight steps' inputs are requested together.
-// 4 x 4096 x 4096 channels, width 4, in 16 bits, full lengths (268 MB, floor 41 us): 59 us.  Eight channels and
-// four steps together, which hold more of the registers for fewer blocks an SM, 92; four and four 62; runs of
-// 64 steps as 32; 16 steps together and partial groups with a condition on every step 83 and more.
+// 4 x 4096 x 4096 channels, width 4, in 16 bits, full lengths, with state, bias and silu (268 MB, floor 41 us): 63.5 us,
+// 67.4 with the new state's inputs held in registers from the start; widths 5, 6, 7, 8 at 2048 steps 47, 49, 51, 62 us
+// (floor 20; 53 for the first three by the kernel of width 8).  In 32 bits 95 us (floor 82).
+// Ways that were slower, against a form that took 59 us without a state: eight channels and four steps together, which
+// hold more of the registers for fewer blocks an SM, 92; four and four 62; runs of 64 steps as 32; 16 steps together
+// and partial groups with a condition on every step 83 and more.
 // 96 single tokens of 4100 channels in 32 bits: 12.3 to 6.2 us, most of it the launch.
 #include <algorithm>
 
@@ -34,16 +37,16 @@ __device__ __forceinline__ float silu(float v) {
 }
 __device__ __forceinline__ double silu(double v) { return v / (1.0 + exp(-v)); }
 
-// K is the width or more: filters are padded in front with zeros, over inputs that are zero there.  Five
-// blocks an SM where the filters and inputs leave the registers for it.  TOGETHER: steps whose inputs are
-// requested together, 8, or 1 for single tokens (with the others' registers and code 10.2 instead of 6.2 us).
+// K: the width.  Every width has its own kernel: a filter that is filled up with zeros multiplies inputs that it
+// does not reach, and 0 times an infinity is NaN.  Five blocks an SM where the filters and inputs leave the
+// registers for it.  TOGETHER: steps whose inputs are requested together, 8, or 1 for single tokens (with the
+// others' registers and code 10.2 instead of 6.2 us).
 template <typename T, int V, int K, int TOGETHER>
 __global__ void __launch_bounds__(kThreads, TOGETHER == 1 ? 1 : K <= 4 && sizeof(T) <= 4 ? 5 : 3) causal_conv_kernel(CausalConvArgs a, int64_t run, int64_t runs) {
     using A = typename Acc<T>::type;
     const int64_t id = (int64_t)blockIdx.x * kThreads + threadIdx.x, across = a.d / V;
     if (id >= across * runs) return;
     const int64_t c = id % across * V, t0 = id / across * run, t1 = min(t0 + run, a.t);
-    const int pad = K - a.k;
     A w[K][V], bias[V];
     if constexpr (V * sizeof(T) >= 8 && K < kMaxConvWidth) {
         // the filters of V channels are K pieces of V values
@@ -62,7 +65,7 @@ __global__ void __launch_bounds__(kThreads, TOGETHER == 1 ? 1 : K <= 4 && sizeof
 #pragma unroll
         for (int j = 0; j < K; ++j)
 #pragma unroll
-            for (int v = 0; v < V; ++v) w[j][v] = j >= pad ? widen(((const T*)a.weight)[(c + v) * a.k + j - pad]) : A(0);
+            for (int v = 0; v < V; ++v) w[j][v] = widen(((const T*)a.weight)[(c + v) * K + j]);
     }
 #pragma unroll
     for (int v = 0; v < V; ++v) bias[v] = a.bias ? widen(((const T*)a.bias)[c + v]) : A(0);
@@ -73,21 +76,21 @@ __global__ void __launch_bounds__(kThreads, TOGETHER == 1 ? 1 : K <= 4 && sizeof
     for (int64_t b = blockIdx.y; b < a.b; b += gridDim.y) {
         const int64_t end = a.lengths ? min(max((int64_t)a.lengths[b], (int64_t)0), a.t) : a.t;
         const T* const xs = (const T*)a.x + b * a.t * a.d + c;
-        const T* const before = a.state ? (const T*)a.state + b * (a.k - 1) * a.d + c : nullptr;
+        const T* const before = a.state ? (const T*)a.state + b * (K - 1) * a.d + c : nullptr;
         T* const ys = (T*)a.y + b * a.t * a.d + c;
-        T* const after = (T*)a.new_state + b * (a.k - 1) * a.d + c;
+        T* const after = (T*)a.new_state + b * (K - 1) * a.d + c;
         auto input = [&](int64_t t) -> Pack<T, V> {
             if (t >= 0) return *(const Pack<T, V>*)(xs + t * a.d);
-            return before && t + a.k - 1 >= 0 ? *(const Pack<T, V>*)(before + (t + a.k - 1) * a.d) : zero;
+            return before ? *(const Pack<T, V>*)(before + (t + K - 1) * a.d) : zero;
         };
-        // the first run's threads carry the state: read before, written behind everything else, since
-        // it may be the same array for a single step
+        // the first run's threads carry the state: for a single step, where it may be the same array, read before
+        // and written behind everything else; for longer ones read there too, which holds no registers
         Pack<T, V> keep[K - 1];
-        if (t0 == 0) {
+        auto carry = [&]() {
 #pragma unroll
-            for (int j = 0; j < K - 1; ++j)
-                if (j < a.k - 1) keep[j] = input(end - a.k + 1 + j);
-        }
+            for (int j = 0; j < K - 1; ++j) keep[j] = input(end - K + 1 + j);
+        };
+        if (TOGETHER == 1 && t0 == 0) carry();
         const int64_t live = min(t1, end);
         int64_t t = t0;
         if (t < live) {
@@ -145,9 +148,9 @@ __global__ void __launch_bounds__(kThreads, TOGETHER == 1 ? 1 : K <= 4 && sizeof
         }
         for (; t < t1; ++t) *(Pack<T, V>*)(ys + t * a.d) = zero;
         if (t0 == 0) {
+            if (TOGETHER != 1) carry();
 #pragma unroll
-            for (int j = 0; j < K - 1; ++j)
-                if (j < a.k - 1) *(Pack<T, V>*)(after + j * a.d) = keep[j];
+            for (int j = 0; j < K - 1; ++j) *(Pack<T, V>*)(after + j * a.d) = keep[j];
         }
     }
 }
@@ -173,7 +176,11 @@ cudaError_t conv(const CausalConvArgs& a, int sm_count, cudaStream_t s) {
         case 2: return conv<T, V, 2>(a, sm_count, s);
         case 3: return conv<T, V, 3>(a, sm_count, s);
         case 4: return conv<T, V, 4>(a, sm_count, s);
-        default: return conv<T, V, kMaxConvWidth>(a, sm_count, s);
+        case 5: return conv<T, V, 5>(a, sm_count, s);
+        case 6: return conv<T, V, 6>(a, sm_count, s);
+        case 7: return conv<T, V, 7>(a, sm_count, s);
+        case kMaxConvWidth: return conv<T, V, kMaxConvWidth>(a, sm_count, s);
+        default: return cudaErrorInvalidValue;
     }
 }
 

@@ -1,0 +1,42 @@
+"""GPU tests of the sequence model operators where values are infinite or NaN, against the CPU oracle."""
+import numpy as np
+import pytest
+
+import charmnumeric_b200 as cnp
+from oracle import sequence as S
+from tests.helpers import run_both
+from tests.test_gpu_sequence import TYPES
+
+pytestmark = pytest.mark.gpu
+
+
+# ---- causal_conv --------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("d", [24, 6, 5])
+@pytest.mark.parametrize("k", range(2, 9))
+def test_causal_conv_infinities_reach_as_far_as_the_filter(interface, k, d, dtype):
+    """One infinity or NaN in the inputs or the state shows in k outputs, across the borders of runs too, and in
+    no other.  Small whole numbers: every sum is exact."""
+    rng = np.random.default_rng(k + d)
+    x = rng.integers(-3, 4, (3, 100, d)).astype(dtype)
+    state = rng.integers(-3, 4, (3, k - 1, d)).astype(dtype)
+    w = rng.choice([-3, -2, -1, 1, 2, 3], (d, k)).astype(dtype)
+    for at, c, v in ((3, 1, np.inf), (31, 2, np.nan), (70, 3, -np.inf), (63, d - 1, np.inf), (99, 0, np.nan)):
+        x[0, at, c] = v
+    state[1, 0, 0], state[1, k - 2, d - 1], state[2, :, 1] = np.inf, np.nan, -np.inf
+    lengths = np.array([100, 40, 7], np.int32)
+
+    def program():
+        ax, aw, ast = (cnp.asarray(v) for v in (x, w, state))
+        y1, s1 = cnp.causal_conv(ax, aw, state=ast)
+        y2, s2 = cnp.causal_conv(ax, aw, state=ast, lengths=lengths)
+        y3, s3 = cnp.causal_conv(cnp.asarray(x[:, 3:4].copy()), aw, state=ast)
+        return {"y1": y1, "s1": s1, "y2": y2, "s2": s2, "y3": y3, "s3": s3}
+    gpu, _ = run_both(interface, program)
+    with np.errstate(invalid="ignore"):
+        want = {"1": S.causal_conv(x, w, None, state, None, 0), "2": S.causal_conv(x, w, None, state, lengths, 0),
+                "3": S.causal_conv(x[:, 3:4], w, None, state, None, 0)}
+    for i, (y, s) in want.items():
+        np.testing.assert_array_equal(gpu["y" + i], y)
+        np.testing.assert_array_equal(gpu["s" + i], s)
