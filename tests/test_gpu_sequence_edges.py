@@ -5,7 +5,7 @@ import pytest
 import charmnumeric_b200 as cnp
 from oracle import sequence as S
 from tests.helpers import run_both
-from tests.test_gpu_sequence import TYPES
+from tests.test_gpu_sequence import TYPES, acc, run_scan
 
 pytestmark = pytest.mark.gpu
 
@@ -40,3 +40,36 @@ def test_causal_conv_infinities_reach_as_far_as_the_filter(interface, k, d, dtyp
     for i, (y, s) in want.items():
         np.testing.assert_array_equal(gpu["y" + i], y)
         np.testing.assert_array_equal(gpu["s" + i], s)
+
+
+# ---- selective_scan -----------------------------------------------------------------------------------------
+
+def flat_inputs(b, t, d, n, dtype, **more):
+    """Every value 1 and every decay e^-dt: all sums have one sign, so that an infinity meets no other."""
+    f = acc(dtype)
+    a = {"x": np.ones((b, t, d), dtype), "delta": np.zeros((b, t, d), dtype), "A": -np.ones((d, n), f),
+         "B": np.ones((b, t, n), dtype), "C": np.ones((b, t, n), dtype)}
+    return dict(a, **more)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("t", [1, 40, 700])
+@pytest.mark.parametrize("n", [1, 2, 3, 5, 8, 12, 16, 20, 31, 40, 64, 100, 128, 200, 256])
+def test_selective_scan_infinities(interface, n, t, dtype):
+    """Infinite inputs and step sizes: infinite from there on in their channel, whatever the number of states is
+    filled up to, with D and without, gated and not."""
+    f = acc(dtype)
+    a = flat_inputs(2, t, 9, n, dtype)
+    a["x"][0, t // 2, 3] = np.inf
+    a["x"][1, t - 1, 8] = np.inf
+    a["delta"][1, t // 3, 5] = np.inf
+    with_d, gated = dict(a, D=np.ones(9, f)), dict(a, z=np.ones_like(a["x"]))
+
+    def program():
+        return {k + i: v for i, inputs in (("0", a), ("1", with_d), ("2", gated)) for k, v in zip("ys", run_scan(inputs))}
+    gpu, cpu = run_both(interface, program)
+    for i in "012":
+        for k in "ys":
+            np.testing.assert_array_equal(np.isinf(gpu[k + i]), np.isinf(cpu[k + i]), err_msg=k + i)
+            assert not np.isnan(gpu[k + i]).any()
+        assert np.isinf(cpu["y" + i][0, t // 2:, 3]).all() and np.isinf(cpu["y" + i]).sum() == (t - t // 2) + 1 + (t - t // 3)
