@@ -77,6 +77,17 @@ template <> __device__ __forceinline__ float decay_scale<float>() { return 1.442
 __device__ __forceinline__ float decay_of(float dt, float a) { return power(fmaf(dt, a, 1.44e-8f)); }
 __device__ __forceinline__ double decay_of(double dt, double a) { return exp(dt * a); }
 
+// A state v behind steps that multiply it by 2^e (e^e for doubles) in all.  The power may leave the type's range where
+// the product does not, nor the steps one by one: it is then taken in two factors, a state of 0 stays 0 and an
+// infinite one infinite.
+template <typename A>
+__device__ __forceinline__ A carried(A e, A v) {
+    if (v == 0 || (fabs(v) == (A)INFINITY && fabs(e) < (A)INFINITY)) return v;
+    if (fabs(e) <= (sizeof(A) == 8 ? A(600) : A(100))) return power(e) * v;
+    const A half = power(e * A(0.5));
+    return half * (half * v);
+}
+
 __device__ __forceinline__ float reciprocal(float v) {
     float r;
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
@@ -264,7 +275,7 @@ __global__ void __launch_bounds__(kThreads + kHelpers, sizeof(T) <= 4 && N == 2 
                         for (int k = 0; k < (int)blockIdx.y; ++k) {
                             const int64_t q = (b * ck.count + k) * a.d;
                             const A s = ck.sums[q + c];
-                            v = (s == 0 ? v : power(w * s) * v) + ck.local[q * a.n + i];
+                            v = (s == 0 ? v : carried(w * s, v)) + ck.local[q * a.n + i];
                         }
                 }
                 (j ? h[p].y : h[p].x) = v;

@@ -5,7 +5,7 @@ import pytest
 import charmnumeric_b200 as cnp
 from oracle import sequence as S
 from tests.helpers import run_both
-from tests.test_gpu_sequence import TYPES, acc, run_scan
+from tests.test_gpu_sequence import TYPES, acc, run_scan, scan_exact
 
 pytestmark = pytest.mark.gpu
 
@@ -73,3 +73,28 @@ def test_selective_scan_infinities(interface, n, t, dtype):
             np.testing.assert_array_equal(np.isinf(gpu[k + i]), np.isinf(cpu[k + i]), err_msg=k + i)
             assert not np.isnan(gpu[k + i]).any()
         assert np.isinf(cpu["y" + i][0, t // 2:, 3]).all() and np.isinf(cpu["y" + i]).sum() == (t - t // 2) + 1 + (t - t // 3)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_selective_scan_decays_beyond_the_range_of_a_type(interface, dtype):
+    """Few channels and many steps, which are walked in pieces: what a piece multiplies an earlier state by may
+    leave the type's range on either side while the product does not."""
+    f = acc(dtype)
+    much = 800.0 if dtype == "float64" else 100.0          # beyond e^88 and e^709
+    b, t, d, n = 1, 640, 4, 3
+    a = flat_inputs(b, t, d, n, dtype)
+    a["delta"] = np.zeros((b, t, d), dtype)
+    a["delta"][0, :64] = 1
+    a["delta"][0, 576:] = 2.0 ** -10
+    a["x"][0, :64] = 0
+    a["A"] = (np.array([[1.0], [-1.0], [1.0], [-1.0]]) * [1.0, 0.5, 0.25] * much / 64).astype(f)
+    a["A"][3] *= 20                                        # 64 steps leave nothing, one of them something
+    large = 1e300 if dtype == "float64" else 1e36
+    a["state"] = np.array([[[0.0] * 3, [large, 1.0, 0.0], [1 / large] * 3, [np.inf, -np.inf, 1.0]]], f)
+    gpu, _ = run_both(interface, lambda: dict(zip("ys", run_scan(dict(a), softplus=False))))
+    with np.errstate(all="ignore"):
+        y, yo, h, ho = scan_exact(dict(a), None, 0)
+    fine = np.isfinite(h)
+    np.testing.assert_array_equal(gpu["s"][~fine], h.astype(f)[~fine])
+    off = np.abs(gpu["s"].astype(float) - np.where(fine, h, 0))
+    assert fine[0, :3].all() and (off <= ho + 2.0 ** -23 * np.abs(np.where(fine, h, 0)))[fine].all()
