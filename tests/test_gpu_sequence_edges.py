@@ -98,3 +98,28 @@ def test_selective_scan_decays_beyond_the_range_of_a_type(interface, dtype):
     np.testing.assert_array_equal(gpu["s"][~fine], h.astype(f)[~fine])
     off = np.abs(gpu["s"].astype(float) - np.where(fine, h, 0))
     assert fine[0, :3].all() and (off <= ho + 2.0 ** -23 * np.abs(np.where(fine, h, 0)))[fine].all()
+
+
+# ---- conversions ----------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("scales", ["float32", "float64"])
+@pytest.mark.parametrize("target", TYPES)
+@pytest.mark.parametrize("n,group", [(2048, 64), (2047, 2047), (2050, 3)])
+def test_dequantize_rounds_once(interface, n, group, target, scales):
+    rng = np.random.default_rng(n)
+    q = rng.integers(-127, 128, (257, n)).astype(np.int8)
+    s = np.exp(rng.uniform(-22, 3, (257, -(-n // group)))).astype(scales)
+    s[0, 0], s[1, 0], s[2, 0], s[3, 0] = 0, np.inf, np.nan, np.finfo(scales).max
+    gpu, _ = run_both(interface, lambda: {"v": cnp.dequantize(cnp.asarray(q), cnp.asarray(s), group=group, dtype=target)})
+    with np.errstate(all="ignore"):
+        # 8 bits times 53 fit the 64 of a long double; to 16 bits through the neighbouring double whose last bit
+        # is 1 where it is not exact, which lies on the same side of every border as the product
+        exact = q.astype(np.longdouble) * np.repeat(s.astype(np.longdouble), group, -1)[:, :n]
+        if target == "float16":
+            near = exact.astype(np.float64)
+            odd = near.view(np.uint64) & np.uint64(1) == 1
+            other = np.nextafter(near, np.where(exact > near, np.inf, -np.inf))
+            exact = np.where((near == exact) | ~np.isfinite(near) | odd, near, other)
+        exact = exact.astype(target)
+    assert np.finfo(np.longdouble).nmant >= 63
+    np.testing.assert_array_equal(gpu["v"], exact)
