@@ -408,9 +408,12 @@ int Context::execute_convert(const DagNode& node) {
     a.in = x.data();
     a.out = out->buf.data;
     a.scale = scale.data();
-    a.rows = n > 0 ? x.a->local_elems() / n : 0;
-    if (a.rows == 0) return CN_OK;
-    prof_start(std::string("convert #") + kSequenceSourceDigest, (double)a.rows * n * (dtype_size(a.from) + dtype_size(a.to)));
+    // rows matter to scales alone; without them a rank converts whatever it has (of a vector, a part of the only row)
+    const int64_t size = x.a->local_elems();
+    if (size == 0) return CN_OK;
+    if (!scale) a.n = size;
+    a.rows = size / a.n;
+    prof_start(std::string("convert #") + kSequenceSourceDigest, (double)size * (dtype_size(a.from) + dtype_size(a.to)));
     rc = cuda_fail(launch_convert(a, sm_count_, stream_), "convert");
     prof_stop();
     if (rc) return rc;

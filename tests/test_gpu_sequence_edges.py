@@ -5,7 +5,7 @@ import pytest
 import charmnumeric_b200 as cnp
 from oracle import sequence as S
 from tests.helpers import run_both
-from tests.test_gpu_sequence import TYPES, acc, run_scan, scan_exact
+from tests.test_gpu_sequence import TYPES, acc, bits, run_scan, scan_exact
 
 pytestmark = pytest.mark.gpu
 
@@ -123,3 +123,68 @@ def test_dequantize_rounds_once(interface, n, group, target, scales):
         exact = exact.astype(target)
     assert np.finfo(np.longdouble).nmant >= 63
     np.testing.assert_array_equal(gpu["v"], exact)
+
+
+# ---- a rank's part --------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("n", [1, 2, 7, 1000, 4099])
+def test_a_rank_converts_its_part_of_a_vector(n):
+    """Each of two ranks' contexts alone: converting needs nothing of the other."""
+    from charmnumeric_b200 import wire
+    x = np.arange(n) * 0.37 - 5
+    parts = []
+    for rank in range(2):
+        ctx = cnp.Context(device=0, rank=rank, nranks=2)
+        try:
+            ctx.put(1, x)
+            for name, code in ((2, wire.F16), (3, wire.I32)):
+                ctx.run([wire.Node(0, [wire.Ast(name, wire.OP_CONVERT, shape=(n,), dtype=code,
+                                                operands=[(wire.leaf(1, (n,), wire.F64), None), (wire.scalar(0.0), None), (wire.scalar(0.0), None)])],
+                                   fusible=False)])
+            ctx.synchronize()
+            (begin, end), half = ctx.get_local(2)
+            _, whole = ctx.get_local(3)
+            bits(half, x[begin:end].astype(np.float16))
+            bits(whole, x[begin:end].astype(np.int32))
+            parts.append(half)
+        finally:
+            ctx.close()
+    if n > 1:
+        bits(np.concatenate(parts), x.astype(np.float16))
+
+
+@pytest.mark.parametrize("rows", [2, 5, 8])
+def test_a_rank_works_on_its_rows(rows):
+    """The operators on two ranks' contexts without parameters to gather: each has its rows of the results."""
+    from charmnumeric_b200 import wire
+    rng = np.random.default_rng(rows)
+    x, u = rng.standard_normal((rows, 300)).astype(np.float32), rng.random(rows).astype(np.float32)
+    whole = S.rms_norm(x, None, None, 1e-6, 0)[0]
+    token = S.sample(x, u, 1.0, 5, 1.0, 0.0)[0]
+    q, s = S.rms_norm(x, None, None, 1e-6, 100)
+    for rank in range(2):
+        ctx = cnp.Context(device=0, rank=rank, nranks=2)
+        try:
+            ctx.put(1, x)
+            ctx.put(2, u)
+            none, lit = (wire.scalar(0.0), None), lambda v: (wire.scalar(v), None)  # noqa: E731
+            ax, au = (wire.leaf(1, x.shape, wire.F32), None), (wire.leaf(2, u.shape, wire.F32), None)
+            noop = lambda name, shape, code: wire.Ast(name, wire.OP_NOOP, shape=shape, dtype=code)  # noqa: E731
+            nodes = [wire.Node(0, [wire.Ast(3, wire.OP_RMS_NORM, shape=x.shape, dtype=wire.F32, operands=[ax, none, none, lit(1e-6), none])], fusible=False),
+                     wire.Node(1, [wire.Ast(4, wire.OP_SAMPLE, shape=(rows,), dtype=wire.I32, operands=[ax, au, lit(1.0), lit(5.0), lit(1.0), none]),
+                                   noop(5, (rows,), wire.F32)], fusible=False),
+                     wire.Node(2, [wire.Ast(6, wire.OP_RMS_NORM, shape=x.shape, dtype=wire.I8, operands=[ax, none, none, lit(1e-6), lit(100.0)]),
+                                   noop(7, (rows, 3), wire.F32)], fusible=False),
+                     wire.Node(3, [wire.Ast(8, wire.OP_CONVERT, shape=x.shape, dtype=wire.F32, operands=[
+                         (wire.leaf(6, x.shape, wire.I8), None), (wire.leaf(7, (rows, 3), wire.F32), None), lit(100.0)])], fusible=False)]
+            ctx.run(nodes)
+            ctx.synchronize()
+            (b, e), y = ctx.get_local(3)
+            np.testing.assert_allclose(y, whole[b:e], rtol=30 * 2.0 ** -24)
+            np.testing.assert_array_equal(ctx.get_local(4)[1], token[b:e])
+            bits(ctx.get_local(6)[1], q[b:e])
+            got = ctx.get_local(7)[1]
+            np.testing.assert_allclose(got, s[b:e], rtol=30 * 2.0 ** -24)
+            np.testing.assert_array_equal(ctx.get_local(8)[1], ctx.get_local(6)[1] * np.repeat(got, 100, -1))
+        finally:
+            ctx.close()
