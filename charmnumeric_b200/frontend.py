@@ -952,7 +952,7 @@ def _group_node(g, consumers_outside):
     for op in g.ops:
         if op.kind == "ew":
             res = op.result
-            temp = (not res.alive) and res.name not in consumers_outside
+            temp = not res.alive and not res.pins and res.name not in consumers_outside
             roots.append(wire.Ast(res.name, op.opcode, is_temp=temp, shape=res.shape,
                                   dtype=WIRE_DTYPES[res.dtype],
                                   operands=[_operand_ast(o, produced, res.dtype) for o in op.operands]))

@@ -188,3 +188,19 @@ def test_a_rank_works_on_its_rows(rows):
             np.testing.assert_array_equal(ctx.get_local(8)[1], ctx.get_local(6)[1] * np.repeat(got, 100, -1))
         finally:
             ctx.close()
+
+
+# ---- steps and other libraries' memory ------------------------------------------------------------------------
+
+def test_a_step_built_by_a_helper(interface):
+    """Its operands are results that nothing has computed yet when the helper returns."""
+    rng = np.random.default_rng(5)
+    x, w = rng.standard_normal((3, 40)), rng.standard_normal((40,))
+
+    def helper():
+        h, s = cnp.asarray(x) * 2.0 + 1.0, cnp.exp(cnp.asarray(w))
+        return cnp.record(lambda: cnp.rms_norm(h, s))
+    step = helper()
+    want = S.rms_norm(x * 2.0 + 1.0, np.exp(w), None, 1e-6, 0)[0]
+    for _ in range(3):
+        np.testing.assert_allclose(step.run(interface).get(interface), want, rtol=1e-13)

@@ -1,0 +1,64 @@
+"""CPU tests of recorded steps: what a step uses exists when it runs, and is released with it."""
+import gc
+
+import charmnumeric_b200 as cnp
+from charmnumeric_b200 import frontend as F, wire
+
+
+def leaves(node):
+    return {leaf.result_name for root in node.roots for leaf, _ in root.operands if isinstance(leaf, wire.Ast) and not leaf.is_scalar}
+
+
+class Backend:
+    """An interface and its context that keep the names of the arrays a backend would have."""
+
+    def __init__(self):
+        self.context = self
+        self.arrays, self.steps = set(), 0
+
+    def run(self, nodes, deletes=()):
+        for node in nodes:
+            assert leaves(node) <= self.arrays
+            self.arrays |= {r.result_name for r in node.roots if not r.is_temp and r.opcode != wire.OP_SET_REGION}
+        self.arrays -= set(deletes)
+
+    def put(self, name, host):
+        self.arrays.add(name)
+
+    def receive_dag(self, blob):
+        self.steps += 1
+
+
+def record(fn, monkeypatch):
+    """cnp.record, and the names of the arrays that the step reads and does not make."""
+    nodes, build = [], F.build_nodes
+
+    def watch(ops):
+        items = build(ops)
+        nodes.extend(node for _, node in items)
+        return items
+    with monkeypatch.context() as m:
+        m.setattr(F, "build_nodes", watch)
+        step = cnp.record(fn)
+    made = {r.result_name for node in nodes for r in node.roots}
+    return step, set().union(*(leaves(node) for node in nodes)) - made
+
+
+def test_a_step_keeps_results_that_are_not_made_yet(monkeypatch):
+    """The operands of a step that a helper returns: pending elementwise results without a handle."""
+    backend = Backend()
+
+    def helper():
+        x, w = cnp.asarray([[1.0, 2.0], [3.0, 4.0]]) * 2.0 + 1.0, cnp.exp(cnp.ones((2,)))
+        return record(lambda: cnp.rms_norm(x, w), monkeypatch)
+    step, used = helper()
+    gc.collect()
+    assert len(used) == 2
+    for _ in range(2):
+        step.run(backend)
+        assert used <= backend.arrays
+    assert backend.steps == 2
+    del step
+    gc.collect()
+    cnp.execute(backend)
+    assert not used & backend.arrays
