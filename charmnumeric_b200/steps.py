@@ -26,6 +26,9 @@ class Step:
         self._blob = wire.dag_blob(nodes)
         for info in infos:
             info.pins += 1
+        # one that the recorded function let go of waits to be released: _unpin does that now
+        kept = {info.name for info in infos}
+        F._state.dead[:] = [name for name in F._state.dead if name not in kept]
         weakref.finalize(self, _unpin, infos)
 
     def run(self, interface):

@@ -204,3 +204,18 @@ def test_a_step_built_by_a_helper(interface):
     want = S.rms_norm(x * 2.0 + 1.0, np.exp(w), None, 1e-6, 0)[0]
     for _ in range(3):
         np.testing.assert_allclose(step.run(interface).get(interface), want, rtol=1e-13)
+
+
+def test_a_step_that_lets_go_of_its_input(interface):
+    x = np.random.default_rng(6).standard_normal((3, 40))
+    h = cnp.asarray(x)
+    cnp.execute(interface)
+
+    def fn():
+        nonlocal h
+        h = cnp.rms_norm(h)
+        return h
+    step = cnp.record(fn)
+    want = S.rms_norm(x, None, None, 1e-6, 0)[0]
+    for _ in range(3):
+        np.testing.assert_allclose(step.run(interface).get(interface), want, rtol=1e-13)

@@ -62,3 +62,25 @@ def test_a_step_keeps_results_that_are_not_made_yet(monkeypatch):
     gc.collect()
     cnp.execute(backend)
     assert not used & backend.arrays
+
+
+def test_a_step_keeps_what_its_function_lets_go_of(monkeypatch):
+    """`h = rms_norm(h)` inside: the last handle on the operand goes while the step is recorded."""
+    backend = Backend()
+    h = cnp.asarray([[1.0, 2.0], [3.0, 4.0]])
+    cnp.execute(backend)
+
+    def fn():
+        nonlocal h
+        h = cnp.rms_norm(h)
+        gc.collect()
+        return h
+    step, used = record(fn, monkeypatch)
+    assert len(used) == 1
+    for _ in range(2):
+        step.run(backend)
+        assert used <= backend.arrays
+    del step
+    gc.collect()
+    cnp.execute(backend)
+    assert not used & backend.arrays
