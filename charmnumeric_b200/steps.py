@@ -33,7 +33,7 @@ class Step:
 
     def run(self, interface):
         """Run the step once (asynchronously), after everything recorded before."""
-        if F._state.pending or F._state.dead:
+        if F._state.pending or F._state.dead or F._state.recording:    # which execute refuses
             F.execute(interface)
         interface.context.receive_dag(self._blob)
         return self.results
@@ -41,7 +41,7 @@ class Step:
 
 def record(fn):
     """The operations that ``fn()`` records, as a ``Step``.  It must not upload host data,
-    and nothing can be executed or fetched inside."""
+    and nothing can be executed or fetched inside, nor another step run."""
     outer, F._state.pending = F._state.pending, []
     flush, F._state.auto_flush = F._state.auto_flush, None
     within, F._state.recording = F._state.recording, True

@@ -1,6 +1,8 @@
 """CPU tests of recorded steps: what a step uses exists when it runs, and is released with it."""
 import gc
 
+import pytest
+
 import charmnumeric_b200 as cnp
 from charmnumeric_b200 import frontend as F, wire
 
@@ -84,3 +86,16 @@ def test_a_step_keeps_what_its_function_lets_go_of(monkeypatch):
     gc.collect()
     cnp.execute(backend)
     assert not used & backend.arrays
+
+
+def test_a_step_does_not_run_while_another_is_recorded():
+    """It would run once, then and there, and not be part of the recorded step."""
+    backend = Backend()
+    x = cnp.asarray([[1.0, 2.0], [3.0, 4.0]])
+    inner = cnp.record(lambda: cnp.rms_norm(x))
+    cnp.execute(backend)
+    with pytest.raises(RuntimeError):
+        cnp.record(lambda: inner.run(backend))
+    assert backend.steps == 0 and not F._state.recording
+    inner.run(backend)
+    assert backend.steps == 1
