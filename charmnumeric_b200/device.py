@@ -52,4 +52,6 @@ def from_device(interface, source):
     else:
         interface.context.put_device(out.name, shape, dtype, about["data"][0], about.get("stream") or 0)
     out._info.materialised = True
+    if isinstance(source, DeviceView):
+        out._info.group = source.array._info.group
     return out

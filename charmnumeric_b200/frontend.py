@@ -128,7 +128,7 @@ def _size(shape):
 
 class _Info:
     """Identity of one backend array; op records keep these, never the user objects."""
-    __slots__ = ("name", "shape", "dtype", "alive", "materialised", "pins", "__weakref__")
+    __slots__ = ("name", "shape", "dtype", "alive", "materialised", "pins", "group", "__weakref__")
 
     def __init__(self, name, shape, dtype):
         self.name = name
@@ -137,6 +137,7 @@ class _Info:
         self.alive = True          # a user-facing Array / ArrayView still refers to it
         self.materialised = False  # exists in the backend's array table
         self.pins = 0              # recorded steps that use the array
+        self.group = None          # scales of 8-bit codes: columns of each, 0 where assignments left it open
 
 
 class _Op:
@@ -354,6 +355,7 @@ class _ArrayOps:
         dtype = _normalize_dtype(dtype)
         if dtype != self.dtype:
             out = _new_array(self.shape, dtype)
+            out._info.group = _group_of(self)
             _record(_Op("seq", wire.OP_CONVERT, out._info, [_whole(self)._operand(), None, 0], payload=[out._info]))
             return out
         return self.copy() if copy else self
@@ -369,6 +371,7 @@ class _ArrayOps:
         if self._region is not None:
             region = _compose(self._region, region)
         rhs = _coerce_assignment(rhs, region.shape(), self.dtype)
+        _assign_group(self._info, region, rhs)
         if _is_storage(self.dtype) or (isinstance(rhs, _ArrayOps) and _is_storage(rhs.dtype)):
             # no generated kernel takes these: a fill or a copy, its own node
             if not isinstance(rhs, _ArrayOps):
@@ -453,6 +456,28 @@ class ArrayView(_ArrayOps):
         return self.copy().get(interface)
 
 
+def _group_of(a):
+    """Columns that each of these values is the scale of (see ``_Info.group``): those of the array, where
+    all of its last dimension is there."""
+    info, region = a._info, a._region
+    if info.group is None or region is None or (region.start[-1], region.stop[-1], region.step[-1]) == (0, info.shape[-1], 1):
+        return info.group
+    return None
+
+
+def _assign_group(info, region, rhs):
+    group = _group_of(rhs) if isinstance(rhs, _ArrayOps) and rhs._info.group is not None and tuple(rhs.shape) == tuple(region.shape()) else None
+    if group != info.group:
+        info.group = group if info.group is None and region == _full_region(info.shape) else 0
+
+
+def _combined_group(out, *operands):
+    for x in operands:
+        if isinstance(x, _ArrayOps) and x._info.group is not None and x.shape == out.shape:
+            group, info = _group_of(x), out._info
+            info.group = group if info.group in (None, group) else 0
+
+
 def _new_array(shape, dtype):
     return Array(_Info(_state.new_name(), tuple(shape), np.dtype(dtype)))
 
@@ -510,6 +535,7 @@ def _binary(opcode, a, b):
     a, b = _coerce_operand(a), _coerce_operand(b)
     _arithmetic(a, b)
     out = _new_array(_result_shape(a, b), _result_dtype(a, b))
+    _combined_group(out, a, b)
     operands = [x._operand() if isinstance(x, _ArrayOps) else x for x in (a, b)]
     _record(_Op("ew", opcode, out._info, operands))
     return out
@@ -519,6 +545,7 @@ def _unary(opcode, x):
     x = asarray(x)
     _arithmetic(x)
     out = _new_array(x.shape, x.dtype)
+    _combined_group(out, x)
     _record(_Op("ew", opcode, out._info, [x._operand()]))
     return out
 

@@ -83,7 +83,7 @@ def rms_norm(x, weight=None, *, residual=None, eps=1e-6, bits=None, group=None):
     results = [_new_array(x.shape, _I8 if bits else x.dtype)]
     if bits:
         results.append(_new_array(tuple(x.shape[:-1]) + (-(-n // group),), _acc(x)))
-        results[1]._group = group  # so that dequantize need not be told
+        results[1]._info.group = group  # so that dequantize need not be told
     if residual is not None:
         results.append(_new_array(x.shape, x.dtype))
     _apply(wire.OP_RMS_NORM, [x, weight, residual, float(eps), group], results)
@@ -93,7 +93,9 @@ def rms_norm(x, weight=None, *, residual=None, eps=1e-6, bits=None, group=None):
 def dequantize(codes, scale, *, group=None, dtype=None):
     """The values that int8 codes stand for, ``code * scale`` with one scale for every ``group`` columns
     of the last dimension, in ``dtype`` (default: that of the scales).  ``group`` may be left out for scales
-    that ``rms_norm`` returned, and where the columns divide evenly among the scales."""
+    that ``rms_norm`` returned, their copies, conversions, rows and what is computed from them value by value.
+    Scales from elsewhere are taken to have as many columns each as divide evenly: give the group of others (30 of
+    100 columns make four scales, as 25 do)."""
     codes = _operand(codes, "codes", (_I8,), None)
     scale = _operand(scale, "scale", (_F32, _F64), None)
     dtype = scale.dtype if dtype is None else _normalize_dtype(dtype)
@@ -104,8 +106,10 @@ def dequantize(codes, scale, *, group=None, dtype=None):
         raise ValueError(f"scales of shape {tuple(scale.shape)} do not go with codes of shape {tuple(codes.shape)}")
     groups = scale.shape[-1]
     if group is None:
-        group = getattr(scale, "_group", None)
-        if group is None:
+        group = scale._info.group
+        if group == 0 and groups > 1:
+            raise ValueError("give the group: the scales were assigned to, from others that may have another one")
+        if not group:
             if not groups or n % groups:
                 raise ValueError(f"give the group: {n} columns do not divide evenly among {groups} scales")
             group = n // groups

@@ -219,3 +219,17 @@ def test_a_step_that_lets_go_of_its_input(interface):
     want = S.rms_norm(x, None, None, 1e-6, 0)[0]
     for _ in range(3):
         np.testing.assert_allclose(step.run(interface).get(interface), want, rtol=1e-13)
+
+
+def test_scales_keep_their_group(interface):
+    """Groups of 30 of 100 columns make as many scales as groups of 25."""
+    x = np.random.default_rng(7).standard_normal((5, 100)).astype("float32")
+
+    def program():
+        q, s = cnp.rms_norm(cnp.asarray(x), bits=8, group=30)
+        return {"q": q, "s": s, "v": cnp.dequantize(q, s), "copy": cnp.dequantize(q, s.copy()),
+                "view": cnp.dequantize(q, s[:]), "wide": cnp.dequantize(q, s.astype("float64"), dtype="float32")}
+    gpu, _ = run_both(interface, program)
+    want = gpu["q"] * np.repeat(gpu["s"], 30, -1)[:, :100]
+    for k in ("v", "copy", "view", "wide"):
+        np.testing.assert_array_equal(gpu[k], want, err_msg=k)
