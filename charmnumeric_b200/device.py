@@ -26,10 +26,12 @@ def device_view(array, interface):
     return DeviceView(array, (end - begin,) + tuple(array.shape[1:]), pointer, stream)
 
 
-def from_device(interface, source):
+def from_device(interface, source, stream=None):
     """A copy of another library's device array (dense, on the interface's GPU) as an ``Array``.  The copy
-    is ordered behind the stream that ``source`` names, or else the default stream, and that stream
-    behind the copy."""
+    is ordered behind ``stream``, the handle of the stream that the values are made on, and that stream
+    behind the copy.  Without it the stream is the one that ``source`` names in its interface, or else the default
+    stream: give it for tensors of libraries that name none and work on streams of their own (of torch's,
+    ``torch.cuda.current_stream().cuda_stream``)."""
     about = getattr(source, "__cuda_array_interface__", None)
     if about is None:
         raise TypeError(f"{type(source).__name__} has no __cuda_array_interface__")
@@ -50,7 +52,7 @@ def from_device(interface, source):
     if 0 in shape:
         interface.context.put(out.name, np.empty(shape, dtype))
     else:
-        interface.context.put_device(out.name, shape, dtype, about["data"][0], about.get("stream") or 0)
+        interface.context.put_device(out.name, shape, dtype, about["data"][0], int(about.get("stream") or 0) if stream is None else int(stream))
     out._info.materialised = True
     if isinstance(source, DeviceView):
         out._info.group = source.array._info.group

@@ -233,3 +233,23 @@ def test_scales_keep_their_group(interface):
     want = gpu["q"] * np.repeat(gpu["s"], 30, -1)[:, :100]
     for k in ("v", "copy", "view", "wide"):
         np.testing.assert_array_equal(gpu[k], want, err_msg=k)
+
+
+@pytest.mark.parametrize("named", ["argument", "interface"])
+def test_device_memory_made_on_another_stream(interface, named):
+    import torch
+    side = torch.cuda.Stream()
+    t = torch.zeros(1 << 22, device="cuda")
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(50_000_000)                # some 25 ms
+        t += 3
+        if named == "argument":
+            a = cnp.from_device(interface, t, stream=side.cuda_stream)
+        else:
+            class Named:
+                __cuda_array_interface__ = dict(t.__cuda_array_interface__, version=3, stream=side.cuda_stream)
+            a = cnp.from_device(interface, Named())
+        t.zero_()                                      # behind the copy
+    assert (a.get(interface) == 3).all()
+    side.synchronize()
