@@ -163,6 +163,10 @@ def prepare(case, seed):
         torch.cuda.synchronize()
         arrays = {k: None if v is None else cnp.from_device(interface, v) for k, v in inputs.items()}
         interface.context.synchronize()
+        # one stream for both libraries: torch's kernels that read an output run behind the operator that makes it, and
+        # the next pass, which writes it again, behind them
+        stream = next(v for v in arrays.values() if v is not None).device_view(interface).stream
+        torch.cuda.set_stream(torch.cuda.ExternalStream(stream))
         state.update(interface=interface, step=cnp.record(lambda: _OWN[case["op"]](cnp, case, arrays)), out=None)
         state["inputs"] = None
     return state
