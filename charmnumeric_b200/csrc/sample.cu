@@ -516,7 +516,7 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 8 ? 1 : 2) sample_kerne
         };
         auto write = [&](Key k, int at, u64 total) {
             a.token[row] = at;
-            const double e = k == top ? 0.0 : ((double)O::value(k) - (double)most) / (double)temp;
+            const double e = k == top ? 0.0 : ((double)O::value(k) * 0.5 - (double)most * 0.5) / (double)temp * 2.0;    // halves, as in depth()
             ((A*)a.logp)[row] = (A)(e - log((double)total / (double)(1ULL << shift)));
         };
         const A least = (A)fmin(row_param(a.min_p, row), 1.0);   // the largest logit stays

@@ -5,7 +5,7 @@ import pytest
 import charmnumeric_b200 as cnp
 from oracle import sequence as S
 from tests.helpers import run_both
-from tests.test_gpu_sequence import TYPES, acc, bits, run_scan, scan_exact
+from tests.test_gpu_sequence import TYPES, acc, bits, check_samples, run_scan, scan_exact
 
 pytestmark = pytest.mark.gpu
 
@@ -253,3 +253,27 @@ def test_device_memory_made_on_another_stream(interface, named):
         t.zero_()                                      # behind the copy
     assert (a.get(interface) == 3).all()
     side.synchronize()
+
+
+# ---- sample -------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", ["float32", "float64"])
+def test_sample_logits_and_temperatures_at_the_end_of_a_type(interface, dtype):
+    """Logits as large as the type's values over temperatures as large: a few powers of e from end to end, which
+    in the units of the logits leave the type's range."""
+    most = float(np.finfo(dtype).max)
+    rng = np.random.default_rng(23)
+    v = 6000
+    span = np.linspace(-1, 1, v)
+    x = (most * np.stack([span, rng.permutation(span), rng.uniform(-1, 1, v), rng.uniform(-1, 0.25, v)])).astype(dtype)
+    u = np.array([0.2, 0.99, 0.9999, 0.5], dtype)
+    sets = [(most / over, k, p, 0.0) for over in (1.0, 3.4, 10.0, 30.0) for k, p in ((0, 0.9), (0, 0.999), (0, 0.9999), (3000, 1.0), (5500, 0.9999))]
+
+    def program():
+        out, ax, au = {}, cnp.asarray(x), cnp.asarray(u)
+        for i, (t, k, p, m) in enumerate(sets):
+            out[f"t{i}"], out[f"p{i}"] = cnp.random.sample(ax, au, temperature=t, top_k=k, top_p=p, min_p=m)
+        return out
+    gpu, _ = run_both(interface, program)
+    for i, f in enumerate(sets):
+        check_samples(x, gpu[f"t{i}"], gpu[f"p{i}"], u, *f)
