@@ -39,8 +39,14 @@ def _operand(v, what, dtypes, shape):
     if v is None:
         return None
     if not isinstance(v, _ArrayOps):
-        v = np.asarray(v)
-        v = asarray(v if v.dtype in dtypes else v.astype(dtypes[0]))
+        host = np.asarray(v)
+        if host.dtype not in dtypes:
+            with np.errstate(invalid="ignore"):
+                v = host.astype(dtypes[0])
+            if dtypes[0].kind == "i" and not np.array_equal(v, host):
+                raise ValueError(f"{what} must be whole numbers that {dtypes[0]} holds")
+            host = v
+        v = asarray(host)
     if v.dtype not in dtypes:
         raise TypeError(f"{what} must be {' or '.join(d.name for d in dtypes)}, got {v.dtype}")
     if shape is not None and tuple(v.shape) != tuple(shape):
