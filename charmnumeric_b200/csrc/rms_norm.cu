@@ -231,7 +231,10 @@ __global__ void __launch_bounds__(W == 1 ? 128 : W * 32) rms_norm_8_kernel(RmsNo
     }
 }
 
-// Any length, any group, any alignment; a block a row, which is read again for the results.
+// Any length, any group, any alignment; a block a row, which is read again for the results.  The simple kernel, value by
+// value and a warp a group: 8192 rows of 4096 in 16 bits with a residual and their values, groups of 100 226 us, of 512
+// 138, 4097 columns in groups of 128 199 (82 for groups of 128 in registers); 256 rows of 70000 in 32 bits with one scale
+// 2482, of which one warp a row has most.
 template <typename T>
 __global__ void __launch_bounds__(256) rms_norm_long_kernel(RmsNormArgs a) {
     using A = typename Acc<T>::type;

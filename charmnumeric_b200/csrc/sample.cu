@@ -8,6 +8,8 @@
 // A temperature that is not above 0 keeps the first of the largest logits alone.
 // The token is the first in index order whose running sum of kept e exceeds u times their total.
 //
+// A weight is the hardware's 2^x of a 32-bit argument (64 bits and exp2 for 64-bit logits), with a relative error of
+// some 2^-22 + |log2 e| 2^-24: that of a difference of logits in 32 bits.
 // The sums are held as 64-bit integers, e 2^s rounded to one, with s such that no row overflows: they do not
 // depend on the order of the additions, so every way of splitting a row gives the same token, and
 // the first two filters come down to one border in the order of the logits, (key, number of ties kept).

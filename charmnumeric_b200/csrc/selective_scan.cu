@@ -15,11 +15,14 @@
 // 1 x 8192 x 4096 channels x 16 states in 16 bits, gated (floor 119 us at 1.9 GHz): a thread a channel
 // 12332 us; states over lanes, tiles of 16 steps in shared memory 621; lanes' sums through shared memory
 // instead of shuffles 570; walkers and helpers side by side, tiles copied ahead through a ring, sums and
-// B, C in fewer bytes of shared memory 335 us.  There the issue slots are busy two
+// B, C in fewer bytes of shared memory 336 us.  There the issue slots are busy two
 // thirds of the time and the special function units and shared memory half each: what is left is the
 // instructions around an exponential (two steps' B and C widened, the term, the recurrence, C h).
-// 5 x 1003 x 1537 x 16 in 32 bits, of random lengths: 1352 to 94 us (floor 27 at full length).
-// 2 x 1000 x 500 x 12 in 64 bits: 1027 to 104 us (exponentials in FP64 instructions, twice over in chunks).
+// 5 x 1003 x 1537 x 16 in 32 bits, of random lengths: 1352 to 84-107 us (floor 27 at full length).
+// 2 x 1000 x 500 x 12 in 64 bits: 1027 to 106 us (exponentials in FP64 instructions, twice over in chunks).
+//
+// Floats take the hardware's 2^x and 1 / x (errors of some 2^-22 of the value, and that of a 32-bit argument) in the
+// decays, softplus and the gate: the library's functions would be several times the instructions of a step.
 #include <algorithm>
 #include <type_traits>
 

@@ -1,6 +1,7 @@
 // Fills, strided copies and tiles of arrays of the storage types (float16, int8), which have no
-// arithmetic: a value is moved by its size.  Bound by HBM where the innermost dimension is dense;
-// these are set-up paths, and one value a thread and turn is what the other types' copies do too.
+// arithmetic: a value is moved by its size.  Simple kernels: one value a thread and turn, its place found by 64-bit
+// divisions, which bound them.  Half of each row of 4 x 4096 x 8192 copied: 382 us in 16 bits, 0.7 TB/s (floor 41),
+// 377 in 8.
 #include <cuda_fp16.h>
 
 #include <algorithm>

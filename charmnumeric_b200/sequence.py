@@ -68,7 +68,7 @@ def rms_norm(x, weight=None, *, residual=None, eps=1e-6, bits=None, group=None):
     ``(codes, scale, h)``; ``dequantize`` gives the values.  With ``v = h * weight`` and a group's largest
     ``|v|``, a, codes are ``rint(v * (1 / a * 127))``, whatever the row's norm.  A group that is all zero (or
     so small that 1 / a overflows) has codes and scale 0, one with an infinity or a NaN codes 0 and
-    scale NaN.
+    scale NaN.  Squares are summed in float32 (float64 for float64): float32 rows with values beyond 1.8e19 are 0.
     """
     x = _activations(x, "x", (1, 2, 3))
     n = x.shape[-1]
