@@ -55,5 +55,5 @@ def from_device(interface, source, stream=None):
         interface.context.put_device(out.name, shape, dtype, about["data"][0], int(about.get("stream") or 0) if stream is None else int(stream))
     out._info.materialised = True
     if isinstance(source, DeviceView):
-        out._info.group = source.array._info.group
+        out._info.set_group(source.array._info.group)
     return out

@@ -78,14 +78,14 @@ def _normalize_dtype(dtype):
 
 
 def _is_storage(dtype):
-    return dtype in (np.dtype("float16"), np.dtype("int8"))
+    return dtype.itemsize < 4     # float16 and int8
 
 
 def _arithmetic(*arrays):
     """float16 and int8 arrays can be made, filled, assigned, converted and given to the operators
     of sequence models; nothing is computed with them directly."""
     for a in arrays:
-        if isinstance(a, _ArrayOps) and _is_storage(a.dtype):
+        if isinstance(a, _ArrayOps) and a._info.marked and _is_storage(a.dtype):
             raise TypeError(f"{a.dtype} is a storage type: convert the array with astype first")
 
 
@@ -128,7 +128,7 @@ def _size(shape):
 
 class _Info:
     """Identity of one backend array; op records keep these, never the user objects."""
-    __slots__ = ("name", "shape", "dtype", "alive", "materialised", "pins", "group", "__weakref__")
+    __slots__ = ("name", "shape", "dtype", "alive", "materialised", "pins", "group", "marked", "__weakref__")
 
     def __init__(self, name, shape, dtype):
         self.name = name
@@ -138,6 +138,10 @@ class _Info:
         self.materialised = False  # exists in the backend's array table
         self.pins = 0              # recorded steps that use the array
         self.group = None          # scales of 8-bit codes: columns of each, 0 where assignments left it open
+        self.marked = _is_storage(dtype)    # of a storage type, or scales: operations look closer
+
+    def set_group(self, group):
+        self.group, self.marked = group, self.marked or group is not None
 
 
 class _Op:
@@ -355,7 +359,7 @@ class _ArrayOps:
         dtype = _normalize_dtype(dtype)
         if dtype != self.dtype:
             out = _new_array(self.shape, dtype)
-            out._info.group = _group_of(self)
+            out._info.set_group(_group_of(self))
             _record(_Op("seq", wire.OP_CONVERT, out._info, [_whole(self)._operand(), None, 0], payload=[out._info]))
             return out
         return self.copy() if copy else self
@@ -371,8 +375,10 @@ class _ArrayOps:
         if self._region is not None:
             region = _compose(self._region, region)
         rhs = _coerce_assignment(rhs, region.shape(), self.dtype)
-        _assign_group(self._info, region, rhs)
-        if _is_storage(self.dtype) or (isinstance(rhs, _ArrayOps) and _is_storage(rhs.dtype)):
+        marked = self._info.marked or (isinstance(rhs, _ArrayOps) and rhs._info.marked)
+        if marked:
+            _assign_group(self._info, region, rhs)
+        if marked and (_is_storage(self.dtype) or (isinstance(rhs, _ArrayOps) and _is_storage(rhs.dtype))):
             # no generated kernel takes these: a fill or a copy, its own node
             if not isinstance(rhs, _ArrayOps):
                 if self.dtype == np.dtype("int8") and not -128 <= rhs <= 127:
@@ -468,14 +474,14 @@ def _group_of(a):
 def _assign_group(info, region, rhs):
     group = _group_of(rhs) if isinstance(rhs, _ArrayOps) and rhs._info.group is not None and tuple(rhs.shape) == tuple(region.shape()) else None
     if group != info.group:
-        info.group = group if info.group is None and region == _full_region(info.shape) else 0
+        info.set_group(group if info.group is None and region == _full_region(info.shape) else 0)
 
 
 def _combined_group(out, *operands):
     for x in operands:
         if isinstance(x, _ArrayOps) and x._info.group is not None and x.shape == out.shape:
             group, info = _group_of(x), out._info
-            info.group = group if info.group in (None, group) else 0
+            info.set_group(group if info.group in (None, group) else 0)
 
 
 def _new_array(shape, dtype):
@@ -533,10 +539,17 @@ def _result_dtype(a, b):
 
 def _binary(opcode, a, b):
     a, b = _coerce_operand(a), _coerce_operand(b)
-    _arithmetic(a, b)
+    operands, marked = [], False
+    for x in (a, b):
+        if isinstance(x, _ArrayOps):
+            marked = marked or x._info.marked
+            x = (x._info, x._region)
+        operands.append(x)
+    if marked:
+        _arithmetic(a, b)
     out = _new_array(_result_shape(a, b), _result_dtype(a, b))
-    _combined_group(out, a, b)
-    operands = [x._operand() if isinstance(x, _ArrayOps) else x for x in (a, b)]
+    if marked:
+        _combined_group(out, a, b)
     _record(_Op("ew", opcode, out._info, operands))
     return out
 

@@ -89,7 +89,7 @@ def rms_norm(x, weight=None, *, residual=None, eps=1e-6, bits=None, group=None):
     results = [_new_array(x.shape, _I8 if bits else x.dtype)]
     if bits:
         results.append(_new_array(tuple(x.shape[:-1]) + (-(-n // group),), _acc(x)))
-        results[1]._info.group = group  # so that dequantize need not be told
+        results[1]._info.set_group(group)  # so that dequantize need not be told
     if residual is not None:
         results.append(_new_array(x.shape, x.dtype))
     _apply(wire.OP_RMS_NORM, [x, weight, residual, float(eps), group], results)
