@@ -472,9 +472,14 @@ def _group_of(a):
 
 
 def _assign_group(info, region, rhs):
+    """What an array stands for after an assignment.  Rows of scales in other groups have no meaning together:
+    unknown ones are taken to fit, a whole array of them may be of any group."""
     group = _group_of(rhs) if isinstance(rhs, _ArrayOps) and rhs._info.group is not None and tuple(rhs.shape) == tuple(region.shape()) else None
-    if group != info.group:
-        info.set_group(group if info.group is None and region == _full_region(info.shape) else 0)
+    whole = region == _full_region(info.shape)
+    if info.group is None or (whole and group is not None):
+        info.set_group(group)
+    elif group != info.group and (whole or group is not None):
+        info.set_group(0)
 
 
 def _combined_group(out, *operands):

@@ -37,14 +37,14 @@ def test_rows_and_multiples_of_scales():
     np.testing.assert_array_equal(v, 2 * want)
 
 
-@pytest.mark.parametrize("change", ["host", "other", "part", "sum"])
+@pytest.mark.parametrize("change", ["host", "number", "part", "sum"])
 def test_scales_that_were_assigned_to_ask_for_the_group(change):
     q, s = cnp.rms_norm(cnp.asarray(X), bits=8, group=30)
     _, other = cnp.rms_norm(cnp.asarray(X), bits=8, group=25)
     if change == "host":
         s[...] = np.ones((5, 4), "float32")
-    elif change == "other":
-        s[...] = other
+    elif change == "number":
+        s[...] = 1
     elif change == "part":
         s[1:2] = other[1:2]
     else:
@@ -52,6 +52,28 @@ def test_scales_that_were_assigned_to_ask_for_the_group(change):
     with pytest.raises(ValueError):
         cnp.dequantize(q, s)
     cnp.dequantize(q, s, group=25)
+
+
+def test_scales_put_together_from_rows():
+    def parts(s):
+        out = cnp.zeros(s.shape, dtype="float32")
+        out[:2] = s[:2]
+        out[2:] = s[2:]
+        return out
+    v, want = values(parts)
+    np.testing.assert_array_equal(v, want)
+    v, want = values(lambda s: (s.__setitem__(slice(0, 1), np.zeros((1, 4), "float32")), s)[1])
+    np.testing.assert_array_equal(v, want)
+    assert (v[0] == 0).all()
+
+
+def test_scales_assigned_over_others():
+    def over(s):
+        _, other = cnp.rms_norm(cnp.asarray(X), bits=8, group=25)
+        other[...] = s
+        return other
+    v, want = values(over)
+    np.testing.assert_array_equal(v, want)
 
 
 def test_scales_from_elsewhere_divide_evenly():
