@@ -316,7 +316,7 @@ int Context::execute_selective_scan(const DagNode& node) {
         prof_stop();
         if (ws) cudaFreeAsync(ws, stream_);
         if (rc) return rc;
-        stats_.kernel_launches++;
+        stats_.kernel_launches += ws ? 2 : 1;    // pieces of the time axis are walked twice
     }
     if (swap) std::swap(state.a->buf, state.a->shadow);
     if (in_place) state.a->mark_written();

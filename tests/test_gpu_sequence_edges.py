@@ -100,6 +100,17 @@ def test_selective_scan_decays_beyond_the_range_of_a_type(interface, dtype):
     assert fine[0, :3].all() and (off <= ho + 2.0 ** -23 * np.abs(np.where(fine, h, 0)))[fine].all()
 
 
+@pytest.mark.parametrize("t,launches", [(1, 1), (100, 1), (640, 2)])
+def test_selective_scan_counts_its_launches(interface, t, launches):
+    """Few channels: long sequences are walked in pieces, by two kernels."""
+    arrays = {k: cnp.asarray(v) for k, v in flat_inputs(1, t, 4, 3, "float32").items()}
+    cnp.execute(interface)
+    before = interface.context.stats()["kernel_launches"]
+    y, s = cnp.selective_scan(*arrays.values())
+    cnp.execute(interface)
+    assert interface.context.stats()["kernel_launches"] - before == launches
+
+
 # ---- conversions ----------------------------------------------------------------------------------------------
 
 @pytest.mark.parametrize("scales", ["float32", "float64"])
