@@ -242,6 +242,7 @@ private:
     int execute_convert(const DagNode& node);
     struct SeqArg;
     int seq_arg(const DagNode& node, size_t i, SeqArg* out);
+    int seq_names(const DagNode& node, const Array* in_place);
     int seq_result(const DagNode& node, size_t i, int ndims, const int64_t* shape, int dtype, Array** out);
     int seq_whole(std::initializer_list<SeqArg*> args);
     int seq_rows(const Array& x, std::initializer_list<const Array*> operands, std::initializer_list<const Array*> results);

@@ -54,15 +54,28 @@ int Context::seq_arg(const DagNode& node, size_t i, SeqArg* out) {
     return CN_OK;
 }
 
-// Result i of the node (root i).  The array must be none of the operands and none of the other results.
-int Context::seq_result(const DagNode& node, size_t i, int ndims, const int64_t* shape, int dtype, Array** out) {
-    const int name = node.roots[i]->result_name;
-    for (auto& op : node.roots[0]->operands)
-        if (op.leaf && !op.leaf->is_scalar && op.leaf->result_name == name)
+// The results (roots) must be none of the operands and none of each other; with a state that is updated in place the
+// second one is the state itself, which then is no other operand.  Checked before any result is made.
+int Context::seq_names(const DagNode& node, const Array* in_place) {
+    const auto& operands = node.roots[0]->operands;
+    for (size_t i = 0; i < node.roots.size(); ++i) {
+        const int name = node.roots[i]->result_name;
+        size_t own = 0;
+        for (auto& op : operands) own += op.leaf && !op.leaf->is_scalar && op.leaf->result_name == name;
+        if (in_place && i == 1) {
+            if (own > 1) return fail(CN_ERR_HAZARD, "a state that is updated in place is also another operand");
+        } else if (own) {
             return fail(CN_ERR_HAZARD, "a result of this operator is one of its operands");
-    for (size_t j = 0; j < node.roots.size(); ++j)
-        if (j != i && node.roots[j]->result_name == name) return fail(CN_ERR_HAZARD, "two results of this operator are the same array");
-    int rc = create_array(name, ndims, shape, dtype, false, out);
+        }
+        for (size_t j = 0; j < i; ++j)
+            if (node.roots[j]->result_name == name) return fail(CN_ERR_HAZARD, "two results of this operator are the same array");
+    }
+    return CN_OK;
+}
+
+// Result i of the node (root i).
+int Context::seq_result(const DagNode& node, size_t i, int ndims, const int64_t* shape, int dtype, Array** out) {
+    int rc = create_array(node.roots[i]->result_name, ndims, shape, dtype, false, out);
     if (rc) return rc;
     (*out)->mark_written();
     return CN_OK;
@@ -139,6 +152,7 @@ int Context::execute_rms_norm(const DagNode& node) {
     const int64_t group = (int64_t)grp.value;
     const size_t results = 1 + (group > 0) + (res ? 1 : 0);
     if (node.roots.size() != results) return fail(CN_ERR_BAD_BLOB, "RMS_NORM: wrong number of results");
+    if ((rc = seq_names(node, nullptr))) return rc;
     Array *y = nullptr, *scale = nullptr, *h = nullptr;
     if ((rc = seq_result(node, 0, nd, x.a->shape, group > 0 ? DT_I8 : dtype, &y))) return rc;
     if (group > 0) {
@@ -197,13 +211,11 @@ int Context::execute_causal_conv(const DagNode& node) {
     if (state && !has_shape(state.a, {b, k - 1, d})) return fail(CN_ERR_SHAPE_MISMATCH, "CAUSAL_CONV state must be (sequences, width - 1, channels)");
     if (len && !has_shape(len.a, {b})) return fail(CN_ERR_SHAPE_MISMATCH, "CAUSAL_CONV lengths must be (sequences)");
     if (act.value != 0 && act.value != 1) return fail(CN_ERR_INVALID_ARGUMENT, "CAUSAL_CONV activation must be 0 or 1");
+    const bool in_place = state && node.roots[1]->result_name == state.a->name;
+    if ((rc = seq_names(node, in_place ? state.a : nullptr))) return rc;
     Array *y = nullptr, *ns = nullptr;
     if ((rc = seq_result(node, 0, 3, x.a->shape, dtype, &y))) return rc;
     const int64_t sshape[3] = {b, k - 1, d};
-    const bool in_place = state && node.roots[1]->result_name == state.a->name;
-    if (in_place)
-        for (SeqArg* p : all)
-            if (p != &state && p->a == state.a) return fail(CN_ERR_HAZARD, "a state that is updated in place is also another operand");
     if (!in_place && (rc = seq_result(node, 1, 3, sshape, dtype, &ns))) return rc;
     // a prompt's blocks read the old state while others write the new one: it goes into the
     // array's shadow buffer, which then takes its place (as stencil sweeps do)
@@ -273,13 +285,11 @@ int Context::execute_selective_scan(const DagNode& node) {
     if (state && !has_shape(state.a, {b, d, n})) return fail(CN_ERR_SHAPE_MISMATCH, "SELECTIVE_SCAN state must be (sequences, channels, states)");
     if (len && !has_shape(len.a, {b})) return fail(CN_ERR_SHAPE_MISMATCH, "SELECTIVE_SCAN lengths must be (sequences)");
     if (sp.value != 0 && sp.value != 1) return fail(CN_ERR_INVALID_ARGUMENT, "SELECTIVE_SCAN softplus must be 0 or 1");
+    const bool in_place = state && node.roots[1]->result_name == state.a->name;
+    if ((rc = seq_names(node, in_place ? state.a : nullptr))) return rc;
     Array *y = nullptr, *ns = nullptr;
     if ((rc = seq_result(node, 0, 3, x.a->shape, dtype, &y))) return rc;
     const int64_t sshape[3] = {b, d, n};
-    const bool in_place = state && node.roots[1]->result_name == state.a->name;
-    if (in_place)
-        for (SeqArg* p : all)
-            if (p != &state && p->a == state.a) return fail(CN_ERR_HAZARD, "a state that is updated in place is also another operand");
     if (!in_place && (rc = seq_result(node, 1, 3, sshape, acc, &ns))) return rc;
     const bool swap = in_place && t != 1;
     if (swap && (rc = ensure_shadow(state.a))) return rc;
@@ -352,6 +362,7 @@ int Context::execute_sample(const DagNode& node) {
         to[i]->data = par[i].data();
         to[i]->dtype = want;
     }
+    if ((rc = seq_names(node, nullptr))) return rc;
     Array *tok = nullptr, *logp = nullptr;
     const int64_t shape[1] = {rows};
     if ((rc = seq_result(node, 0, 1, shape, DT_I32, &tok))) return rc;
@@ -402,6 +413,7 @@ int Context::execute_convert(const DagNode& node) {
         if (!ok) return fail(CN_ERR_SHAPE_MISMATCH, "CONVERT needs one scale per row and group of columns");
         a.scale_dtype = scale.a->dtype;
     }
+    if ((rc = seq_names(node, nullptr))) return rc;
     Array* out = nullptr;
     if ((rc = seq_result(node, 0, nd, x.a->shape, a.to, &out))) return rc;
     if (scale && (rc = seq_rows(*x.a, {scale.a}, {out}))) return rc;

@@ -136,6 +136,33 @@ def test_dequantize_rounds_once(interface, n, group, target, scales):
     np.testing.assert_array_equal(gpu["v"], exact)
 
 
+# ---- refusals -------------------------------------------------------------------------------------------------
+
+def test_a_refused_node_leaves_its_results_alone(interface):
+    """The second result is an operand, or the first: the first one, an array of another shape, is as it was."""
+    from charmnumeric_b200 import wire
+    from charmnumeric_b200._lib import CnError
+    ctx = interface.context
+    keep = np.arange(5.0, dtype=np.float32)
+    ctx.put(880400, np.ones((2, 3, 4), np.float32))
+    ctx.put(880401, np.ones((4, 2), np.float32))
+    ctx.put(880402, keep)
+    x, w, none = (wire.leaf(880400, (2, 3, 4), wire.F32), None), (wire.leaf(880401, (4, 2), wire.F32), None), (wire.scalar(0.0), None)
+    flat = (wire.leaf(880402, (5,), wire.F32), None)
+    noop = lambda name: wire.Ast(name, wire.OP_NOOP, shape=(1,), dtype=wire.F32)  # noqa: E731
+    conv = wire.Ast(880402, wire.OP_CAUSAL_CONV, shape=(1,), dtype=wire.F32, operands=[x, w, none, none, none, none])
+    norm = wire.Ast(880402, wire.OP_RMS_NORM, shape=(1,), dtype=wire.I8, operands=[x, none, none, none, (wire.scalar(4.0), None)])
+    draw = wire.Ast(880403, wire.OP_SAMPLE, shape=(1,), dtype=wire.I32, operands=[flat, (wire.leaf(880404, (1,), wire.F32), None)] + [none] * 4)
+    ctx.put(880404, np.zeros(1, np.float32))
+    for roots in ([conv, noop(880401)], [conv, noop(880402)], [norm, noop(880400)], [draw, noop(880402)]):
+        with pytest.raises(CnError) as e:
+            ctx.run([wire.Node(0, roots, fusible=False)])
+        assert e.value.status == 11
+        bits(ctx.get(880402), keep)
+    for name in (880400, 880401, 880402, 880404):
+        ctx.delete_array(name)
+
+
 # ---- a rank's part --------------------------------------------------------------------------------------------
 
 @pytest.mark.parametrize("n", [1, 2, 7, 1000, 4099])
