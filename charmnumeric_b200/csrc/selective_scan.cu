@@ -86,9 +86,9 @@ __device__ __forceinline__ double decay_of(double dt, double a) { return exp(dt 
 template <typename A>
 __device__ __forceinline__ A carried(A e, A v) {
     if (v == 0 || (fabs(v) == (A)INFINITY && fabs(e) < (A)INFINITY)) return v;
-    if (fabs(e) <= (sizeof(A) == 8 ? A(600) : A(100))) return power(e) * v;
-    const A half = power(e * A(0.5));
-    return half * (half * v);
+    const bool far = !(fabs(e) <= (sizeof(A) == 8 ? A(600) : A(100)));
+    const A p = power(far ? e * A(0.5) : e);
+    return far ? p * (p * v) : p * v;
 }
 
 __device__ __forceinline__ float reciprocal(float v) {
@@ -500,9 +500,14 @@ __global__ void __launch_bounds__(kThreads + kHelpers, sizeof(T) <= 4 && N == 2 
 #pragma unroll
         for (int i = 0; i < kOwnPairs; ++i) {
             const int k = 2 * i + 1 < kOwn ? 2 * i + 1 : 2 * i, s0 = min(row + 2 * i * kRows, S - 1), s1 = min(row + k * kRows, S - 1);
-            const Two<A> x = {widen(*(const T*)(finish_at + own_at[2 * i])), widen(*(const T*)(finish_at + own_at[k]))};
             y[i] = {lanes_sum<L / 2>(sh.y[buf][s0], slot), lanes_sum<L / 2>(sh.y[buf][s1], slot)};
-            if (a.D) y[i] = fma(both(skip), x, y[i]);
+        }
+        if (a.D) {
+#pragma unroll
+            for (int i = 0; i < kOwnPairs; ++i) {
+                const int k = 2 * i + 1 < kOwn ? 2 * i + 1 : 2 * i;
+                y[i] = fma(both(skip), {widen(*(const T*)(finish_at + own_at[2 * i])), widen(*(const T*)(finish_at + own_at[k]))}, y[i]);
+            }
         }
         if (a.z) {
 #pragma unroll
